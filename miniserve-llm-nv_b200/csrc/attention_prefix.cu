@@ -1,0 +1,235 @@
+// Attention of a batch whose requests share the pages of a long prefix.
+//
+// The requests stand in groups of consecutive ones; the first `prefix` tokens of a group's requests lie in the same pages.  A token at position p
+// sees the keys 0 .. p of its request.  With s_t = scale q . k_t (under a soft cap c tanh(s / c)) the softmax over all t is joined from parts:
+//   part i:   m_i = max s_t,  l_i = sum 2^(s_t' - m_i'),  o_i = sum 2^(s_t' - m_i') v_t / l_i,  lse_i = m_i' + log2 l_i      (s' = s log2 e)
+//   whole:    o = sum_i 2^(lse_i - M) o_i / (sum_i 2^(lse_i - M) + 2^(sink' - M))
+// The keys before the prefix's end are parts of the group: all its tokens and all heads of a key head are rows against one read of the keys and
+// values.  What lies behind the prefix are parts of each request.  Both kinds are cut further along the keys where the rows are few.
+//
+// This file holds the kernel for any head size and type in float32 arithmetic, and the join.
+#include "attention_prefix.cuh"
+
+namespace ms {
+namespace prefix {
+
+// Thread block: sixteen rows of one unit (a group's prefix or a request's own keys) and key head, over its share of the keys; a warp holds four rows, a
+// lane one key of a tile of 32 for the scores and every 32nd column for the values.
+constexpr int kRows = 16, kKeys = 32, kThreads = 128;
+
+// COLUMNS: columns of the values to a lane, ceil(d / 32) or more.
+template <typename T, int COLUMNS>
+__global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, Batch b,
+                                                           int d, float scale, float softcap, Parts parts) {
+  grid_dependency_wait();
+  grid_dependency_launch();
+  extern __shared__ __align__(16) float smem[];
+  const int dp = (d + 3) / 4 * 4, ks_stride = dp + 4;
+  float* q_s = smem;                                 // [kRows][dp]
+  float* k_s = q_s + kRows * dp;                     // [kKeys][dp + 4]
+  float* v_s = k_s + kKeys * ks_stride;              // [kKeys][dp]
+  float* p_s = v_s + kKeys * dp;                     // [kRows][kKeys]
+  const Unit u = unit_of(b, (int)blockIdx.z, parts);
+  const int kv_head = blockIdx.y, group = b.n_q / b.n_kv;
+  const int rows_total = (u.token_end - u.token) * group, row0 = (int)blockIdx.x * kRows;
+  if (row0 >= rows_total) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = (u.key_end - u.key + kKeys - 1) / kKeys, share = (tiles + u.splits - 1) / u.splits;
+  const int tile_lo = u.split * share, tile_hi = min(tiles, tile_lo + share);
+  for (int i = threadIdx.x; i < kRows * dp; i += kThreads) {
+    const int r = i / dp, c = i % dp, row = row0 + r;
+    float v = 0.f;
+    if (row < rows_total && c < d) v = to_float(q[((size_t)(u.token + row / group) * b.n_q + kv_head * group + row % group) * d + c]);
+    q_s[i] = v;
+  }
+  int limit[4];                                      // the last position that the row sees
+  float top[4], sum[4], acc[4][COLUMNS];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = row0 + warp * 4 + r;
+    limit[r] = row < rows_total ? b.positions[u.token + row / group] : -1;
+    top[r] = -INFINITY, sum[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c) acc[r][c] = 0.f;
+  }
+  for (int tile = tile_lo; tile < tile_hi; ++tile) {
+    const int key0 = u.key + tile * kKeys, live = min(kKeys, u.key_end - key0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kKeys * dp; i += kThreads) {
+      const int r = i / dp, c = i % dp;
+      float k = 0.f, v = 0.f;                        // (keys behind the last are zeros: whatever their memory holds is not read)
+      if (r < live && c < d) {
+        const int key = key0 + r;
+        const size_t at = (((size_t)u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d + c;
+        k = to_float(k_pool[at]);
+        v = to_float(v_pool[at]);
+      }
+      k_s[r * ks_stride + c] = k;
+      v_s[i] = v;
+    }
+    __syncthreads();
+    float s[4] = {};
+    for (int c = 0; c < dp; c += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(k_s + lane * ks_stride + c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float4 a = *reinterpret_cast<const float4*>(q_s + (warp * 4 + r) * dp + c);
+        s[r] = fmaf(a.x, k.x, fmaf(a.y, k.y, fmaf(a.z, k.z, fmaf(a.w, k.w, s[r]))));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x = s[r] * scale;
+      if (softcap > 0.f) x = softcap * tanhf(x / softcap);
+      x *= kLog2e;
+      if (lane >= live || key0 + lane > limit[r]) x = -INFINITY;
+      const float updated = fmaxf(top[r], warp_max(x));
+      const float base = updated == -INFINITY ? 0.f : updated;
+      const float factor = exp2f(top[r] - base);     // (0 where nothing was seen)
+      const float p = exp2f(x - base);
+      sum[r] = sum[r] * factor + p;                  // of this lane's keys
+      top[r] = updated;
+      p_s[(warp * 4 + r) * kKeys + lane] = p;
+#pragma unroll
+      for (int c = 0; c < COLUMNS; ++c) acc[r][c] *= factor;
+    }
+    __syncwarp();
+    for (int key = 0; key < live; ++key) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[r] = p_s[(warp * 4 + r) * kKeys + key];
+#pragma unroll
+      for (int c = 0; c < COLUMNS; ++c)
+        if (lane + 32 * c < d) {
+          const float v = v_s[key * dp + lane + 32 * c];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (p[r] != 0.f) acc[r][c] = fmaf(p[r], v, acc[r][c]);           // (a value that no row sees may be anything)
+        }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = row0 + warp * 4 + r;
+    const float total = warp_sum(sum[r]);
+    if (row >= rows_total) continue;
+    const size_t item = (size_t)(u.token + row / group) * b.n_q + kv_head * group + row % group, at = item * parts.count + u.part;
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c)
+      if (lane + 32 * c < d) parts.o[at * d + lane + 32 * c] = acc[r][c] * inv;
+    if (lane == 0) parts.lse[at] = total > 0.f ? top[r] + log2f(total) : -INFINITY;
+  }
+}
+
+// Warp: one (token, head).  A part without keys has weight 0 and its numbers are not read.
+template <typename T, int COLUMNS>
+__global__ void __launch_bounds__(128) join_kernel(Parts parts, int d, int n_q, const int* __restrict__ tokens, const float* __restrict__ sink,
+                                                  int has_sink, T* __restrict__ out) {
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int item = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (item / n_q >= *tokens) return;                // (rows behind the last request stay as they are)
+  const float* lse = parts.lse + (size_t)item * parts.count;
+  const float* o = parts.o + (size_t)item * parts.count * d;
+  float top = -INFINITY;
+  for (int i = lane; i < parts.count; i += 32) top = fmaxf(top, __ldcg(lse + i));
+  top = warp_max(top);
+  float sink2 = -INFINITY;
+  if (has_sink) sink2 = sink != nullptr ? sink[item % n_q] * kLog2e : 0.f;
+  top = fmaxf(top, sink2);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = exp2f(sink2 - base), acc[COLUMNS] = {};
+  for (int i = 0; i < parts.count; ++i) {
+    const float w = exp2f(__ldcg(lse + i) - base);
+    if (w == 0.f) continue;
+    total += w;
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c)
+      if (lane + 32 * c < d) acc[c] = fmaf(w, __ldcg(o + (size_t)i * d + lane + 32 * c), acc[c]);
+  }
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+  for (int c = 0; c < COLUMNS; ++c)
+    if (lane + 32 * c < d) out[(size_t)item * d + lane + 32 * c] = from_float<T>(acc[c] * inv);
+}
+
+template <typename T, int COLUMNS>
+int launch_join(const Parts& parts, int d, int n_q, const int* tokens, int items, const float* sink_scores, int sink, void* out, cudaStream_t stream) {
+  ms::launch(join_kernel<T, COLUMNS>, dim3((items + 3) / 4), dim3(128), 0, stream, parts, d, n_q, tokens, sink_scores, sink, (T*)out);
+  MS_CHECK_LAUNCH("prefix attention (join)");
+  return 0;
+}
+
+template <typename T, int COLUMNS>
+int launch_general(const void* q, const void* k_pool, const void* v_pool, const Batch& b, int d, float scale, float softcap, const Parts& parts, dim3 grid,
+                   cudaStream_t stream) {
+  const int dp = (d + 3) / 4 * 4;
+  const size_t smem = (size_t)(kRows * dp + kKeys * (2 * dp + 4) + kRows * kKeys) * sizeof(float);
+  MS_REQUIRE(allow_shared(general_kernel<T, COLUMNS>, smem) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
+  ms::launch(general_kernel<T, COLUMNS>, grid, dim3(kThreads), smem, stream, (const T*)q, (const T*)k_pool, (const T*)v_pool, b, d, scale, softcap, parts);
+  MS_CHECK_LAUNCH("prefix attention");
+  return 0;
+}
+
+template <typename T, int COLUMNS>
+int attend(const void* q, const void* k_pool, const void* v_pool, const Batch& b, int d, float scale, float softcap, const Parts& parts, dim3 grid, int items,
+           const float* sink_scores, int sink, void* out, cudaStream_t stream) {
+  const int code = launch_general<T, COLUMNS>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, stream);
+  return code != 0 ? code : launch_join<T, COLUMNS>(parts, d, b.n_q, b.query_start + b.n_requests, items, sink_scores, sink, out, stream);
+}
+
+template <typename T>
+int attend_any(const void* q, const void* k_pool, const void* v_pool, const Batch& b, int d, float scale, float softcap, const Parts& parts, dim3 grid,
+               int items, const float* sink_scores, int sink, void* out, cudaStream_t stream) {
+  if (d <= 64) return attend<T, 2>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+  if (d <= 128) return attend<T, 4>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+  if (d <= 256) return attend<T, 8>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+  return attend<T, 16>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+}
+
+}  // namespace prefix
+}  // namespace ms
+
+using namespace ms;
+
+
+
+// Into how many parts a unit's keys are cut: so many that the blocks of `units` (units x key heads x row tiles) times the parts fill the GPU's 148
+// multiprocessors about four deep, a part keeping four tiles or more.
+MS_EXPORT int ms_prefix_attention_parts(int units, int most_keys) {
+  if (units < 1) units = 1;
+  int parts = (4 * 148 + units - 1) / units;
+  const int most = (most_keys + 4 * prefix::kKeys - 1) / (4 * prefix::kKeys);
+  if (parts > most) parts = most;
+  if (parts > 64) parts = 64;
+  return parts < 1 ? 1 : parts;
+}
+
+// q, out [n_tokens, n_q, d] of type dtype; pools [pages, n_kv, page_size, d] of one layer; block_tables [requests, table_stride]; positions [n_tokens];
+// query_start [requests + 1]; context_lens [requests] (lengths after this step's tokens); group_start [groups + 1] (requests; the first is 0, the last
+// the number of requests); prefix_lens [groups].  part_o [n_tokens n_q (prefix_parts + own_parts) d] and part_lse (without d) are float32 scratch.
+// max_query_len, max_group_tokens: upper bounds of a request's and a group's tokens.  sink != 0: one more term of the denominator, e^0 or
+// e^sink_scores[head].
+MS_EXPORT int ms_prefix_attention(const void* q, int dtype, const void* k_pool, const void* v_pool, const int* block_tables, int table_stride,
+                                  const int* positions, const int* query_start, const int* context_lens, const int* group_start,
+                                  const int* prefix_lens, int page_size, int n_q, int n_kv, int d, float scale, float softcap, int sink,
+                                  const float* sink_scores, void* out, float* part_o, float* part_lse, int prefix_parts, int own_parts, int n_requests,
+                                  int n_groups, int n_tokens, int max_query_len, int max_group_tokens, cudaStream_t stream) {
+  using namespace ms::prefix;
+  if (n_tokens == 0) return 0;
+  MS_REQUIRE(n_kv > 0 && n_q % n_kv == 0, "prefix attention: %d query heads are not a multiple of %d key/value heads", n_q, n_kv);
+  MS_REQUIRE(d >= 1 && d <= 512 && page_size > 0, "prefix attention: head size %d, page size %d", d, page_size);
+  MS_REQUIRE(prefix_parts >= 0 && own_parts >= 1 && part_o && part_lse, "prefix attention: %d + %d parts need scratch", prefix_parts, own_parts);
+  const long long units = (long long)n_groups * prefix_parts + (long long)n_requests * own_parts;
+  const int group = n_q / n_kv, most = max_query_len > max_group_tokens ? max_query_len : max_group_tokens;
+  const long long tiles = ((long long)most * group + kRows - 1) / kRows;
+  MS_REQUIRE(units <= 65535 && n_kv <= 65535 && tiles <= 2147483647LL, "prefix attention: grid %lld x %d x %lld exceeds the launch limits", tiles, n_kv, units);
+  const Batch b{block_tables, table_stride, positions, query_start, context_lens, group_start, prefix_lens, page_size, n_q, n_kv, n_requests, n_groups};
+  const Parts parts{part_o, part_lse, prefix_parts, own_parts, prefix_parts + own_parts};
+  const dim3 grid((unsigned)tiles, n_kv, (unsigned)units);
+  const int items = n_tokens * n_q;
+  if (dtype == MS_F32) return attend_any<float>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+  return attend_any<__nv_bfloat16>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
+}

@@ -1,0 +1,80 @@
+// What the kernels of attention behind a shared prefix have in common: the batch, its units of work and where their parts of the result go.
+#pragma once
+
+#include "common.cuh"
+
+namespace ms {
+namespace prefix {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Batch {
+  const int* block_tables;
+  int table_stride;
+  const int* positions;
+  const int* query_start;
+  const int* context_lens;
+  const int* group_start;
+  const int* prefix_lens;
+  int page_size, n_q, n_kv, n_requests, n_groups;
+};
+
+// Results of parts: o [items][count][d] and lse [items][count] in base 2, item = token * n_q + head; a unit's split i of a prefix is part i, of a
+// request's own keys part prefix + i.
+struct Parts {
+  float* o;
+  float* lse;
+  int prefix, own, count;
+};
+
+struct Unit {
+  int token, token_end;      // the rows' tokens
+  int key, key_end;          // all of the unit's keys
+  const int* table;
+  int split, splits, part;
+};
+
+__device__ __forceinline__ int group_of(const Batch& b, int request) {
+  int low = 0, high = b.n_groups - 1;             // the last group that starts at or before the request
+  while (low < high) {
+    const int mid = (low + high + 1) / 2;
+    if (b.group_start[mid] <= request) low = mid; else high = mid - 1;
+  }
+  return low;
+}
+
+// The keys that a group reads from its first request's table: never more than that request has.
+__device__ __forceinline__ int prefix_of(const Batch& b, int group) {
+  const int leader = b.group_start[group];
+  const int most = leader < b.n_requests ? b.context_lens[leader] : 0;
+  return max(0, min(b.prefix_lens[group], most));
+}
+
+__device__ __forceinline__ Unit prefix_unit(const Batch& b, int group, int split, const Parts& parts) {
+  Unit u;
+  const int first = b.group_start[group], last = min(b.group_start[group + 1], b.n_requests);
+  u.token = b.query_start[first], u.token_end = max(u.token, b.query_start[last]);
+  u.key = 0, u.key_end = prefix_of(b, group);
+  u.table = b.block_tables + (size_t)first * b.table_stride;
+  u.split = split, u.splits = parts.prefix, u.part = split;
+  return u;
+}
+
+__device__ __forceinline__ Unit own_unit(const Batch& b, int request, int split, const Parts& parts) {
+  Unit u;
+  u.token = b.query_start[request], u.token_end = b.query_start[request + 1];
+  u.key = prefix_of(b, group_of(b, request)), u.key_end = max(u.key, b.context_lens[request]);
+  u.table = b.block_tables + (size_t)request * b.table_stride;
+  u.split = split, u.splits = parts.own, u.part = parts.prefix + split;
+  return u;
+}
+
+// Units in the order: every group's prefix with its splits, then every request's own keys with theirs.
+__device__ __forceinline__ Unit unit_of(const Batch& b, int index, const Parts& parts) {
+  const int shared = b.n_groups * parts.prefix;
+  if (index < shared) return prefix_unit(b, index / parts.prefix, index % parts.prefix, parts);
+  return own_unit(b, (index - shared) / parts.own, (index - shared) % parts.own, parts);
+}
+
+}  // namespace prefix
+}  // namespace ms

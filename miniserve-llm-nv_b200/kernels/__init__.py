@@ -8,19 +8,20 @@ built or loaded, raises.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import importlib.machinery
 import importlib.util
 import logging
 import math
-from typing import Optional, Union
+from typing import Optional, Sequence, Union
 
 import torch
 
 from . import build
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 log = logging.getLogger("miniserve_b200")
 _library: Optional[ctypes.CDLL] = None
 
@@ -126,6 +127,16 @@ def _want(tensor: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise KernelError(f"{name} must be {dtype}, got {tensor.dtype}")
     if shape is not None and tuple(tensor.shape) != tuple(shape):
         raise KernelError(f"{name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}")
+
+
+def _want_here(**tensors: Optional[torch.Tensor]) -> None:
+    """All of them on the current device, whose streams the launches go to."""
+    current = torch.cuda.current_device()
+    for name, tensor in tensors.items():
+        if tensor is not None and tensor.is_cuda and tensor.get_device() != current:
+            raise KernelError(f"{name} lies on {tensor.device}, the current device is cuda:{current}")
+    if _device_index not in (None, current):
+        raise KernelError(f"the library's launches go to cuda:{_device_index}, the current device is cuda:{current}")
 
 
 _i = int        # (arguments are converted by ctypes from the prototypes' types; these only coerce)
@@ -2418,6 +2429,176 @@ def gated_linear(gate_up: torch.Tensor, weight: torch.Tensor, out: torch.Tensor)
     hidden = torch.empty((m, inter), dtype=gate_up.dtype, device=gate_up.device)
     silu_mul(gate_up, hidden)
     linear(hidden, weight, out)
+
+
+# --------------------------------------------------------------------------- many continuations of one prompt
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor, positions: torch.Tensor,
+                            query_start: torch.Tensor, context_lens: torch.Tensor, group_start: torch.Tensor, prefix_lens: torch.Tensor,
+                            max_query_len: int, max_group_tokens: int, max_prefix_len: int, max_suffix_len: int, scale: float,
+                            out: torch.Tensor, softcap: Optional[float] = None, sink: Union[bool, torch.Tensor] = False) -> None:
+    """:func:`paged_attention` for a batch whose requests share the pages of a long prefix: what they share is read once for a group, not once
+    for a request.
+
+    Requests ``group_start[g] .. group_start[g + 1] - 1`` (int32 ``[G + 1]``, from 0 to the number of requests) form group g: the first
+    ``prefix_lens[g]`` (int32 ``[G]``) tokens of each of them lie in the same pages, those that its first request's row of ``block_tables``
+    names (or in copies with the same contents); a prefix is no longer than any of its requests' contexts, and 0 for requests that share nothing.  Whatever stands in the pages behind a
+    request's context is not read as a number (NaN there changes nothing).
+
+    q, out ``[N, n_q, d]`` and pools ``[pages, n_kv, page_size, d]`` of one type, float32 or bfloat16; ``positions`` int32 ``[N]``;
+    ``block_tables``, ``query_start``, ``context_lens``, ``softcap`` and ``sink`` as in :func:`paged_attention`; every key of a prefix is kept
+    (no window).  Upper bounds that shape the grids, which a captured launch keeps: ``max_query_len`` and ``max_group_tokens``, the
+    most tokens of a request and of a group; ``max_prefix_len`` and ``max_suffix_len``, the most keys of a prefix and of a request behind it.
+    A part's share of the keys depends on these bounds, and with it the rounding of the result."""
+    if q.dim() != 3 or k_pool.dim() != 4:
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)} are not [N, n_q, d] or the pool {tuple(k_pool.shape)} is not [pages, n_kv, page_size, d]")
+    n, n_q, head_dim = q.shape
+    n_kv = k_pool.shape[1]
+    n_requests, n_groups = context_lens.numel(), prefix_lens.numel()
+    _want(q, "q")
+    _want(k_pool, "k_pool", q.dtype)
+    if k_pool.shape[3] != head_dim or n_kv < 1 or n_q % n_kv or k_pool.shape[2] < 1:
+        raise KernelError(f"pool shape {tuple(k_pool.shape)} is not [pages, a divisor of {n_q}, page_size, {head_dim}]")
+    _want(v_pool, "v_pool", q.dtype, k_pool.shape)
+    _want(out, "out", q.dtype, (n, n_q, head_dim))
+    if block_tables.dim() != 2 or block_tables.shape[0] != n_requests:
+        raise KernelError(f"block_tables {tuple(block_tables.shape)} for {n_requests} requests")
+    _want(block_tables, "block_tables", torch.int32)
+    _want(positions, "positions", torch.int32, (n,))
+    _want(query_start, "query_start", torch.int32, (n_requests + 1,))
+    _want(context_lens, "context_lens", torch.int32, (n_requests,))
+    _want(group_start, "group_start", torch.int32, (n_groups + 1,))
+    _want(prefix_lens, "prefix_lens", torch.int32, (n_groups,))
+    sink_scores = None
+    if isinstance(sink, torch.Tensor):
+        _want(sink, "sink", torch.float32, (n_q,))
+        sink, sink_scores = True, sink
+    _want_here(q=q, k_pool=k_pool, v_pool=v_pool, block_tables=block_tables, positions=positions, query_start=query_start,
+               context_lens=context_lens, group_start=group_start, prefix_lens=prefix_lens, sink=sink_scores, out=out)
+    if not 1 <= head_dim <= MAX_HEAD_DIM:
+        raise KernelError(f"head size {head_dim} is not in 1..{MAX_HEAD_DIM}")
+    if min(max_query_len, max_group_tokens) < 0 or min(max_prefix_len, max_suffix_len) < 0 or max_group_tokens < max_query_len:
+        raise KernelError(f"shared_prefix_attention: at most {max_query_len} tokens of a request, {max_group_tokens} of a group, {max_prefix_len} keys of a "
+                          f"prefix and {max_suffix_len} behind it")
+    if softcap is not None and not softcap >= 0.0:
+        raise KernelError(f"softcap {softcap} is negative")
+    if n == 0:
+        return
+    if n_requests == 0 or n_groups == 0:
+        raise KernelError(f"{n} tokens of {n_requests} requests in {n_groups} groups")
+    lib = library()
+    group = n_q // n_kv
+    prefix_parts = 0
+    if max_prefix_len > 0:
+        prefix_parts = _asked("ms_prefix_attention_parts", n_groups * n_kv * ((max_group_tokens * group + 15) // 16), max_prefix_len)
+    own_parts = _asked("ms_prefix_attention_parts", n_requests * n_kv * ((max_query_len * group + 15) // 16), max_suffix_len)
+    parts = prefix_parts + own_parts
+    part_o = torch.empty((n * n_q * parts, head_dim), dtype=torch.float32, device=q.device)
+    part_lse = torch.empty((n * n_q * parts,), dtype=torch.float32, device=q.device)
+    _check(lib.ms_prefix_attention(
+        _ptr(q), _i(_code(q.dtype)), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables), _i(block_tables.shape[1]), _ptr(positions),
+        _ptr(query_start), _ptr(context_lens), _ptr(group_start), _ptr(prefix_lens), _i(k_pool.shape[2]), _i(n_q), _i(n_kv), _i(head_dim),
+        _f(scale), _f(softcap or 0.0), _i(1 if sink else 0), _ptr(sink_scores), _ptr(out), _ptr(part_o), _ptr(part_lse), _i(prefix_parts),
+        _i(own_parts), _i(n_requests), _i(n_groups), _i(n), _i(max_query_len), _i(max_group_tokens), _stream()))
+
+
+MAX_COPIED_POOLS = 8
+
+
+def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], sources: Sequence[int], destinations: Sequence[int]) -> None:
+    """``pool[run, destinations[i]] = pool[run, sources[i]]`` for every run of each pool ``[runs, pages, ...]`` and every i, in place: whole pages of a
+    cache to other places (a request that is forked, a pool that is compacted).
+
+    The page numbers are the host's, as the cache's bookkeeping holds them; they travel with the launch (and stay as they are in a captured one).
+    All pools have the same number of pages; types and sizes of a page may differ.  No page is written twice and none is both read
+    and written; one page may be copied to many."""
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if not 1 <= len(pools) <= MAX_COPIED_POOLS:
+        raise KernelError(f"copy_pages: {len(pools)} pools in one call (1..{MAX_COPIED_POOLS})")
+    if isinstance(sources, torch.Tensor) or isinstance(destinations, torch.Tensor):
+        raise KernelError("copy_pages: page numbers are the host's (a list), not a tensor")
+    described = array.array("q")
+    for index, pool in enumerate(pools):
+        name = f"pools[{index}]"
+        _want(pool, name)
+        _want_here(**{name: pool})
+        if pool.dim() < 3 or pool.shape[1] != pools[0].shape[1] or pool.numel() == 0:
+            raise KernelError(f"{name} {tuple(pool.shape)} is not [runs, {pools[0].shape[1]} pages, ...]")
+        described.extend((pool.data_ptr(), pool.shape[0], pool.shape[1], pool.stride(1) * pool.element_size()))
+    try:
+        source, destination = array.array("i", sources), array.array("i", destinations)
+    except (TypeError, OverflowError) as error:
+        raise KernelError(f"copy_pages: page numbers are integers: {error}") from None
+    n, pages = len(source), pools[0].shape[1]
+    if len(destination) != n:
+        raise KernelError(f"copy_pages: {n} sources for {len(destination)} destinations")
+    if n == 0:
+        return
+    if min(source) < 0 or max(source) >= pages or min(destination) < 0 or max(destination) >= pages:
+        raise KernelError(f"copy_pages: a page outside the pool of {pages}")
+    written = set(destination)
+    if len(written) != n:
+        raise KernelError("copy_pages: a page is written twice")
+    if not written.isdisjoint(source):
+        raise KernelError("copy_pages: a page is both read and written")
+    _check(library().ms_copy_pages(described.buffer_info()[0], _i(len(pools)), source.buffer_info()[0], destination.buffer_info()[0], _i(n),
+                                   _stream()))
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, draft_start: torch.Tensor, uniforms: Optional[torch.Tensor],
+                  noise: Optional[torch.Tensor], accepted: torch.Tensor, next_token: torch.Tensor,
+                  draft_probs: Optional[torch.Tensor] = None, records: Optional[torch.Tensor] = None,
+                  slot_of_request: Optional[torch.Tensor] = None, target_probs: Optional[torch.Tensor] = None) -> None:
+    """Checks drafted tokens against the target: how many of each request's are kept, and the token that follows them.
+
+    Request r drafted the tokens ``drafts[draft_start[r]] .. drafts[draft_start[r + 1] - 1]`` (int32 ``[T]`` and ``[R + 1]``, from 0 to T; a request may have
+    none).  ``logits`` float32 ``[T + R, V]`` holds, request after request, the target's rows for its drafts and one for the token behind
+    them.  The target's distribution p of a row is the one that :func:`sample` draws from with the request's record
+    (``records[slot_of_request[r]]``: temperature, top_k, top_p; ``records=None``: argmax for all).
+
+    Draft i passes iff ``uniforms[i] * q_i(drafts[i]) < p_i(drafts[i])``, q the draft's probabilities (``draft_probs`` float32 ``[T, V]``, or None
+    for drafts that were not drawn: one at the drafted token); with temperature 0 iff it is the argmax.  ``accepted`` (int32 ``[R]``) receives the number of
+    drafts that pass before the first that does not, ``next_token`` (int32 ``[R]``) the token after them: at a draft that does not pass the argmax of
+    ``max(p - q, 0) / noise[r]``, where all pass that of ``p / noise[r]`` of the last row, the lowest index among equal ones; with
+    ``uniforms`` (float32 ``[T]``) uniform in [0, 1) and ``noise`` (float32 ``[R, V]``) exponential variates the tokens are then distributed as drawn from
+    p one by one.  With temperature 0 it is the argmax.  Where p - q is positive nowhere, p itself is drawn from.  ``target_probs`` (float32 ``[T]``, or None)
+    receives ``p_i(drafts[i])``.  A logit that is NaN counts as masked (-inf); a row that is masked throughout accepts nothing and gives token 0;
+    a drafted token outside the vocabulary does not pass."""
+    if logits.dim() != 2:
+        raise KernelError(f"verify_drafts: logits {tuple(logits.shape)} are not [rows, vocabulary]")
+    rows, vocab = logits.shape
+    total, requests = drafts.numel(), accepted.numel()
+    _want(logits, "logits", torch.float32)
+    if rows != total + requests or (rows and vocab < 1):
+        raise KernelError(f"verify_drafts: {rows} rows of {vocab} logits for {total} drafts of {requests} requests")
+    _want(drafts, "drafts", torch.int32, (total,))
+    _want(draft_start, "draft_start", torch.int32, (requests + 1,))
+    _want(accepted, "accepted", torch.int32, (requests,))
+    _want(next_token, "next_token", torch.int32, (requests,))
+    if draft_probs is not None:
+        _want(draft_probs, "draft_probs", torch.float32, (total, vocab))
+    if target_probs is not None:
+        _want(target_probs, "target_probs", torch.float32, (total,))
+    if records is not None:
+        _want(records, "records", torch.int32)
+        if records.dim() != 2 or records.shape[1] != SAMPLING_RECORD_WORDS:
+            raise KernelError(f"records must be [slots, {SAMPLING_RECORD_WORDS}] int32")
+        if slot_of_request is None or uniforms is None or noise is None:
+            raise KernelError("verify_drafts: sampling records need slot_of_request, uniforms and noise")
+        _want(slot_of_request, "slot_of_request", torch.int32, (requests,))
+    if uniforms is not None:
+        _want(uniforms, "uniforms", torch.float32, (total,))
+    if noise is not None:
+        _want(noise, "noise", torch.float32, (requests, vocab))
+    _want_here(logits=logits, drafts=drafts, draft_start=draft_start, uniforms=uniforms, noise=noise, accepted=accepted, next_token=next_token,
+               draft_probs=draft_probs, records=records, slot_of_request=slot_of_request, target_probs=target_probs)
+    if requests == 0:
+        return
+    scratch = torch.empty(rows * _asked("ms_verify_row_bytes"), dtype=torch.uint8, device=logits.device)
+    _check(library().ms_verify_drafts(
+        _ptr(logits), _i(vocab), _ptr(drafts), _ptr(draft_start), _i(requests), _i(total), _ptr(uniforms), _ptr(noise), _ptr(draft_probs),
+        _ptr(records), _ptr(slot_of_request), _ptr(accepted), _ptr(next_token), _ptr(target_probs), _ptr(scratch), _stream()))
 
 
 # --------------------------------------------------------------------------- sampling
