@@ -59,6 +59,19 @@ class PageAllocator:
             return True
         return False
 
+    def compact(self) -> dict[int, int]:
+        """Gives the pages in use the lowest numbers: ``{old number: new number}`` of those that move (highest first, each to the lowest free one);
+        their holders come along.  No new number is an old one of the same call."""
+        used = [page for page, count in enumerate(self._refcount) if count]
+        moves: dict[int, int] = {}
+        free = [page for page in range(len(used)) if not self._refcount[page]]
+        for target, page in zip(free, reversed(used)):
+            moves[page] = target
+            self._refcount[target], self._refcount[page] = self._refcount[page], 0
+        if moves:
+            self._free_heap = list(range(len(used), self.num_pages))         # (sorted: a heap)
+        return moves
+
     def check_invariants(self) -> None:
         free = sorted(self._free_heap)
         if len(set(free)) != len(free):

@@ -23,7 +23,7 @@ from typing import Optional, Sequence
 from ..parts.base import PAGED_NEEDS, StateNeed
 from .allocator import OutOfPagesError, PageAllocator
 from .prefix import PrefixCache, PrefixEntry
-from .state_slots import StateSlots
+from .state_slots import OutOfSlotsError, StateSlots
 
 RELEASED = -1   # block-table entry of a page that a sliding window has passed
 
@@ -34,6 +34,7 @@ class RequestCache:
     slot: int
     length: int = 0
     tables: list[list[int]] = field(default_factory=list)   # per paged group: page per page index, or RELEASED
+    changes: int = 0        # counts what changed committed pages (dropped or moved ones): who keeps a copy of a table looks at it
 
 
 @dataclass
@@ -44,6 +45,14 @@ class ReservedItem:
     new_pages: list[list[int]]      # per paged group
     tables: list[list[int]]         # per paged group: the table this step runs with (old + new pages)
     slots: list                     # per paged group: page * page_size + offset of every new token (a numpy array)
+
+
+@dataclass
+class PageCopies:
+    """Whole pages of one paged group to copy: ``sources[i]`` to ``destinations[i]``; no destination is a source."""
+
+    sources: list[int]
+    destinations: list[int]
 
 
 @dataclass
@@ -195,6 +204,61 @@ class CacheManager:
                 self.allocators[group].release(page)
             del table[keep:]
         entry.length = length
+        entry.changes += 1
+
+    # ------------------------------------------------------------------ forks and moves
+    def fork(self, request_id: str, new_ids: Sequence[str]) -> list[PageCopies]:
+        """Admits ``new_ids`` as continuations of the request as it stands: they share its full pages, and each gets a page of its own for the tokens
+        behind the last full one.  Returns per paged group the page copies to make before any of them runs
+        (:meth:`.storage.CacheStorage.copy_pages`).  All or nothing.  Not for groups with a sliding window or
+        models with per-request state, as :meth:`truncate`."""
+        if self._open is not None:
+            raise RuntimeError("a step is open; commit or abort first")
+        parent = self.requests[request_id]
+        if any(not need.keeps_all for need in self.paged_needs) or self.state_needs:
+            raise RuntimeError("fork needs every token's keys and no per-request state")
+        new_ids = list(new_ids)
+        for new_id in new_ids:
+            if new_id in self.requests or new_ids.count(new_id) > 1:
+                raise RuntimeError(f"request {new_id!r} is already admitted")
+        if len(new_ids) > self.slots.free_count:
+            raise OutOfSlotsError(f"{len(new_ids)} forks of request {request_id!r}, {self.slots.free_count} free state slots")
+        full, partial = divmod(parent.length, self.page_size)
+        if partial:
+            self._make_room([len(new_ids)] * len(self.allocators))
+        copies = [PageCopies([], []) for _ in self.allocators]
+        for new_id in new_ids:
+            entry = self.admit(new_id)
+            for group, table in enumerate(parent.tables):
+                for page in table[:full]:
+                    self.allocators[group].retain(page)
+                entry.tables[group].extend(table[:full])
+                if partial:
+                    own = self.allocators[group].allocate(1)[0]
+                    entry.tables[group].append(own)
+                    copies[group].sources.append(table[full])
+                    copies[group].destinations.append(own)
+            entry.length = parent.length
+        return copies
+
+    def compact(self) -> list[PageCopies]:
+        """Gives the pages in use the lowest numbers of each pool, so that a pool's first ``used_count`` pages are all that it holds (one slice to
+        save or to hand on).  Tables and cached prefixes name the new places at once; returns per paged group the copies to make before the next step."""
+        if self._open is not None:
+            raise RuntimeError("a step is open; commit or abort first")
+        copies = []
+        for group, allocator in enumerate(self.allocators):
+            moves = allocator.compact()
+            copies.append(PageCopies(list(moves), list(moves.values())))
+            if not moves:
+                continue
+            for entry in self.requests.values():
+                entry.tables[group] = [moves.get(page, page) for page in entry.tables[group]]
+                entry.changes += 1
+            if self.prefix is not None:
+                for cached in self.prefix.entries.values():
+                    cached.pages = tuple(moves.get(page, page) if g == group else page for g, page in enumerate(cached.pages))
+        return copies
 
     # ------------------------------------------------------------------ capacity
     def pages_for(self, start: int, end: int) -> int:

@@ -18,10 +18,12 @@ from typing import Sequence
 
 import torch
 
+from .. import kernels
 from ..kernels import SAMPLING_RECORD_WORDS
 from ..parts.base import PAGED_NEEDS, PagedKVNeed, PagedLatentNeed, StateNeed
 from ..parts.context import PagedKVView, PagedLatentView, StateView, StepContext
 from ..parts.model import CacheGroup, RunCache
+from .manager import PageCopies
 
 
 class CacheStorage:
@@ -93,6 +95,18 @@ class CacheStorage:
             block_tables, slots = ctx.group_views[self.paged_index[plan.group]]
             return PagedLatentView(self.key_pools[plan.group][plan.slot], block_tables, slots, self.page_size, plan.writable)
         return StateView(self.states[plan.group][plan.slot])
+
+    def copy_pages(self, copies: Sequence[PageCopies]) -> None:
+        """Makes the copies that :meth:`.manager.CacheManager.fork` or :meth:`~.manager.CacheManager.compact` asks for (one entry per paged group), on
+        the current stream: keys and values or latent vectors of all runs, one launch for a group."""
+        of_group = [index for index, paged in enumerate(self.paged_index) if paged is not None]
+        if len(copies) != len(of_group):
+            raise ValueError(f"copies for {len(copies)} paged groups; there are {len(of_group)}")
+        for index, wanted in zip(of_group, copies):
+            if wanted.sources and max(max(wanted.sources), max(wanted.destinations)) >= self.num_pages:
+                raise ValueError(f"a page outside the pool of {self.num_pages}")          # (the scratch page behind them is nobody's)
+            pools = [pool for pool in (self.key_pools[index], self.value_pools[index]) if pool is not None]
+            kernels.copy_pages(pools, wanted.sources, wanted.destinations)
 
     def reset_slot(self, slot: int, temperature: float, top_p: float, top_k: int, seed: int) -> None:
         """Zeroes the slot's state tensors and writes its sampling record (at admission)."""

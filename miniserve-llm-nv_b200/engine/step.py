@@ -60,7 +60,8 @@ class DecodeGraph:
         self.host_np = self.host.numpy()             # same memory, cheaper to fill from Python lists
         self.live_rows = -1
         self.copied: Optional[torch.cuda.Event] = None     # recorded after the last copy of the host mirror
-        # per row: (the request's cache record, pages of its committed table that the mirror shows, per group)
+        # per row: (the request's cache record, pages of its committed table that the mirror shows, per group, pages given back, per
+        # group, and the record's count of changes to committed pages)
         self.row_owner: list = [None] * rows
         # groups whose pages can be given back behind a window or a chunk: a row's table may change anywhere between two steps
         self.gives_back = [not need.keeps_all for need in manager.paged_needs]
@@ -224,6 +225,22 @@ class StepFunction:
             host_query_start=query_start, host_context_lens=context_lens, host_state_slots=state_slots,
             group_views=group_views)
 
+    # ------------------------------------------------------------------ forks and moves of what the cache holds
+    def fork(self, request_id: str, new_ids: Sequence[str]) -> None:
+        """Continuations of a request as it stands (samples of one prompt, drafts to compare): ``new_ids`` share its full pages and get a copy
+        of the page that is partly filled.  Their sampling records are the caller's to write (``storage.reset_slot``)."""
+        copies = self.manager.fork(request_id, new_ids)
+        try:
+            self.storage.copy_pages(copies)
+        except BaseException:
+            for new_id in new_ids:
+                self.manager.release(new_id)
+            raise
+
+    def compact(self) -> None:
+        """Moves the pages in use to the front of their pools."""
+        self.storage.copy_pages(self.manager.compact())
+
     # ------------------------------------------------------------------ running
     def replays(self, entries: Sequence[StepEntry]) -> bool:
         """Whether these entries run as a captured graph: single tokens, all of whose logits are wanted."""
@@ -304,7 +321,7 @@ class StepFunction:
             # The row keeps what it shows only for the very same admission (a request id can come back after a
             # release, with other pages), and only as far as the pages were committed when they were written:
             # a page reserved for a step that was aborted may be another one next time.
-            same = owner is not None and owner[0] is record
+            same = owner is not None and owner[0] is record and owner[3] == record.changes
             released_now = []
             for g in range(graph.n_groups):
                 table = item.tables[g]
@@ -335,7 +352,8 @@ class StepFunction:
                 if not 0 <= slot < limit * ps:
                     raise ValueError(f"slot {slot} outside the pool")
                 host[o[9 + 2 * g] + row] = slot
-            graph.row_owner[row] = (record, [len(item.tables[g]) - len(item.new_pages[g]) for g in range(graph.n_groups)], released_now)
+            graph.row_owner[row] = (record, [len(item.tables[g]) - len(item.new_pages[g]) for g in range(graph.n_groups)], released_now,
+                                    record.changes)
         host[o[0]:o[0] + n] = tokens
         host[o[1]:o[1] + n] = positions
         host[o[4]:o[4] + n] = lens
