@@ -115,11 +115,11 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__
     const float total = warp_sum(sum[r]);
     if (row >= rows_total) continue;
     const size_t item = (size_t)(u.token + row / group) * b.n_q + kv_head * group + row % group, at = item * parts.count + u.part;
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total == 0.f ? 0.f : 1.f / total;          // (NaN stays NaN)
 #pragma unroll
     for (int c = 0; c < COLUMNS; ++c)
       if (lane + 32 * c < d) parts.o[at * d + lane + 32 * c] = acc[r][c] * inv;
-    if (lane == 0) parts.lse[at] = total > 0.f ? top[r] + log2f(total) : -INFINITY;
+    if (lane == 0) parts.lse[at] = total == 0.f ? -INFINITY : top[r] + log2f(total);
   }
 }
 
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(128) join_kernel(Parts parts, int d, int n_q, 
     for (int c = 0; c < COLUMNS; ++c)
       if (lane + 32 * c < d) acc[c] = fmaf(w, __ldcg(o + (size_t)i * d + lane + 32 * c), acc[c]);
   }
-  const float inv = total > 0.f ? 1.f / total : 0.f;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
   for (int c = 0; c < COLUMNS; ++c)
     if (lane + 32 * c < d) out[(size_t)item * d + lane + 32 * c] = from_float<T>(acc[c] * inv);
@@ -196,14 +196,36 @@ using namespace ms;
 
 
 
-// Into how many parts a unit's keys are cut: so many that the blocks of `units` (units x key heads x row tiles) times the parts fill the GPU's 148
-// multiprocessors about four deep, a part keeping four tiles or more.
-MS_EXPORT int ms_prefix_attention_parts(int units, int most_keys) {
-  if (units < 1) units = 1;
-  int parts = (4 * 148 + units - 1) / units;
-  const int most = (most_keys + 4 * prefix::kKeys - 1) / (4 * prefix::kKeys);
+// Whether the tensor-core kernels take the sizes (bfloat16, 16-byte aligned tensors); the general kernel takes all.
+MS_EXPORT int ms_prefix_attention_on_tensor_cores(int d) { return prefix::prefix_mma_takes(d) ? 1 : 0; }
+
+// Into how many parts a unit's keys are cut.  own: the units are `units` requests with up to most_tokens tokens and most_keys keys of their own, else
+// groups and their prefixes.  tensor: on the tensor cores.
+MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int n_kv, int page_size, int units, int most_tokens, int most_keys) {
+  if (units < 1 || n_kv < 1 || most_keys < 1) return 1;
+  const int group = n_q / n_kv;
+  const long long rows = (long long)most_tokens * group;
+  int parts = 1, most = 64;
+  if (tensor && !own && prefix::prefix_tcgen05_takes(d, group, page_size, 0)) {
+    // One block a multiprocessor: what costs least of the blocks' rounds times (a part's tiles + 3, about what a block takes to start and to end), and a
+    // little for every part's results.
+    const int tokens = 128 / group;
+    const long long base = (long long)units * n_kv * ((most_tokens + tokens - 1) / tokens), tiles = (most_keys + 127) / 128;
+    double least = 1e30;
+    for (int s = 1; s <= most && s <= tiles; ++s) {
+      const double cost = (double)((base * s + 147) / 148) * (double)((tiles + s - 1) / s + 3) + 0.1 * s;
+      if (cost < least) least = cost, parts = s;
+    }
+    return parts;
+  }
+  // small blocks: so many that they fill the multiprocessors, a part keeping two tiles or more
+  const bool few = rows <= 16;
+  const long long base = (long long)units * n_kv * (tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
+  const long long slots = 148 * (tensor ? (few ? 5 : 2) : 4);
+  const int keep = tensor ? (few ? 64 : 128) : 128;
+  parts = (int)((slots + base - 1) / base);
+  if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;
   if (parts > most) parts = most;
-  if (parts > 64) parts = 64;
   return parts < 1 ? 1 : parts;
 }
 
@@ -211,12 +233,12 @@ MS_EXPORT int ms_prefix_attention_parts(int units, int most_keys) {
 // query_start [requests + 1]; context_lens [requests] (lengths after this step's tokens); group_start [groups + 1] (requests; the first is 0, the last
 // the number of requests); prefix_lens [groups].  part_o [n_tokens n_q (prefix_parts + own_parts) d] and part_lse (without d) are float32 scratch.
 // max_query_len, max_group_tokens: upper bounds of a request's and a group's tokens.  sink != 0: one more term of the denominator, e^0 or
-// e^sink_scores[head].
-MS_EXPORT int ms_prefix_attention(const void* q, int dtype, const void* k_pool, const void* v_pool, const int* block_tables, int table_stride,
+// e^sink_scores[head].  tensor: the tensor-core kernels are to run (bfloat16, addresses that are multiples of 16 bytes, sizes that they take).
+MS_EXPORT int ms_prefix_attention(int tensor, const void* q, int dtype, const void* k_pool, const void* v_pool, int n_pages, const int* block_tables, int table_stride,
                                   const int* positions, const int* query_start, const int* context_lens, const int* group_start,
                                   const int* prefix_lens, int page_size, int n_q, int n_kv, int d, float scale, float softcap, int sink,
                                   const float* sink_scores, void* out, float* part_o, float* part_lse, int prefix_parts, int own_parts, int n_requests,
-                                  int n_groups, int n_tokens, int max_query_len, int max_group_tokens, cudaStream_t stream) {
+                                  int n_groups, int n_tokens, int max_query_len, int max_group_tokens, int* error_flag, cudaStream_t stream) {
   using namespace ms::prefix;
   if (n_tokens == 0) return 0;
   MS_REQUIRE(n_kv > 0 && n_q % n_kv == 0, "prefix attention: %d query heads are not a multiple of %d key/value heads", n_q, n_kv);
@@ -230,6 +252,19 @@ MS_EXPORT int ms_prefix_attention(const void* q, int dtype, const void* k_pool, 
   const Parts parts{part_o, part_lse, prefix_parts, own_parts, prefix_parts + own_parts};
   const dim3 grid((unsigned)tiles, n_kv, (unsigned)units);
   const int items = n_tokens * n_q;
+  if (tensor) {
+    MS_REQUIRE(dtype == MS_BF16 && prefix_mma_takes(d) && error_flag != nullptr, "prefix attention: head size %d is not the tensor-core kernels'", d);
+    int code = 0;
+    const bool shared = prefix_parts > 0 && n_groups > 0;
+    if (shared && prefix_tcgen05_takes(d, group, page_size, (long long)n_pages * n_kv * page_size))
+      code = launch_prefix_tcgen05(q, k_pool, v_pool, n_pages, b, parts, d, n_tokens, max_group_tokens, scale, softcap, error_flag, stream);
+    else if (shared)
+      code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_group_tokens, scale, softcap, false, false, stream);
+    if (code == 0) code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_query_len, scale, softcap, true, shared, stream);
+    if (code != 0) return code;
+    if (d <= 64) return launch_join<__nv_bfloat16, 2>(parts, d, n_q, query_start + n_requests, items, sink_scores, sink, out, stream);
+    return launch_join<__nv_bfloat16, 4>(parts, d, n_q, query_start + n_requests, items, sink_scores, sink, out, stream);
+  }
   if (dtype == MS_F32) return attend_any<float>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
   return attend_any<__nv_bfloat16>(q, k_pool, v_pool, b, d, scale, softcap, parts, grid, items, sink_scores, sink, out, stream);
 }

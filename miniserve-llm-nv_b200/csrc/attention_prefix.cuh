@@ -76,5 +76,14 @@ __device__ __forceinline__ Unit unit_of(const Batch& b, int index, const Parts& 
   return own_unit(b, (index - shared) / parts.own, (index - shared) % parts.own, parts);
 }
 
+// Launches of the parts on the tensor cores (attention_prefix_tcgen05.cu: prefixes; attention_prefix_mma.cu: prefixes and own keys) and whether they take
+// the sizes; `beside`: see there.
+bool prefix_tcgen05_takes(int d, int group, int page_size, long long pool_rows);
+int launch_prefix_tcgen05(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int n_tokens,
+                          int max_group_tokens, float scale, float softcap, int* error_flag, cudaStream_t stream);
+bool prefix_mma_takes(int d);
+int launch_part_mma(const void* q, const void* k_pool, const void* v_pool, const Batch& b, const Parts& parts, int d, int most_tokens, float scale,
+                    float softcap, bool own, bool beside, cudaStream_t stream);
+
 }  // namespace prefix
 }  // namespace ms

@@ -2483,24 +2483,27 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                           f"prefix and {max_suffix_len} behind it")
     if softcap is not None and not softcap >= 0.0:
         raise KernelError(f"softcap {softcap} is negative")
+    if not 0.0 < scale < math.inf:
+        raise KernelError(f"scale {scale} is not a positive number")
     if n == 0:
         return
     if n_requests == 0 or n_groups == 0:
         raise KernelError(f"{n} tokens of {n_requests} requests in {n_groups} groups")
     lib = library()
-    group = n_q // n_kv
-    prefix_parts = 0
-    if max_prefix_len > 0:
-        prefix_parts = _asked("ms_prefix_attention_parts", n_groups * n_kv * ((max_group_tokens * group + 15) // 16), max_prefix_len)
-    own_parts = _asked("ms_prefix_attention_parts", n_requests * n_kv * ((max_query_len * group + 15) // 16), max_suffix_len)
+    tensor = int(q.dtype is torch.bfloat16 and bool(_asked("ms_prefix_attention_on_tensor_cores", head_dim))
+                 and (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16 == 0)
+    sizes = (tensor, head_dim, n_q, n_kv, k_pool.shape[2])
+    prefix_parts = _asked("ms_prefix_attention_parts", 0, *sizes, n_groups, max_group_tokens, max_prefix_len) if max_prefix_len > 0 else 0
+    own_parts = _asked("ms_prefix_attention_parts", 1, *sizes, n_requests, max_query_len, max_suffix_len)
     parts = prefix_parts + own_parts
     part_o = torch.empty((n * n_q * parts, head_dim), dtype=torch.float32, device=q.device)
     part_lse = torch.empty((n * n_q * parts,), dtype=torch.float32, device=q.device)
     _check(lib.ms_prefix_attention(
-        _ptr(q), _i(_code(q.dtype)), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables), _i(block_tables.shape[1]), _ptr(positions),
-        _ptr(query_start), _ptr(context_lens), _ptr(group_start), _ptr(prefix_lens), _i(k_pool.shape[2]), _i(n_q), _i(n_kv), _i(head_dim),
-        _f(scale), _f(softcap or 0.0), _i(1 if sink else 0), _ptr(sink_scores), _ptr(out), _ptr(part_o), _ptr(part_lse), _i(prefix_parts),
-        _i(own_parts), _i(n_requests), _i(n_groups), _i(n), _i(max_query_len), _i(max_group_tokens), _stream()))
+        _i(tensor), _ptr(q), _i(_code(q.dtype)), _ptr(k_pool), _ptr(v_pool), _i(k_pool.shape[0]), _ptr(block_tables), _i(block_tables.shape[1]),
+        _ptr(positions), _ptr(query_start), _ptr(context_lens), _ptr(group_start), _ptr(prefix_lens), _i(k_pool.shape[2]), _i(n_q), _i(n_kv),
+        _i(head_dim), _f(scale), _f(softcap or 0.0), _i(1 if sink else 0), _ptr(sink_scores), _ptr(out), _ptr(part_o), _ptr(part_lse),
+        _i(prefix_parts), _i(own_parts), _i(n_requests), _i(n_groups), _i(n), _i(max_query_len), _i(max_group_tokens),
+        _ptr(device_error_flag(q.device)), _stream()))
 
 
 MAX_COPIED_POOLS = 8

@@ -276,7 +276,7 @@ def test_refusals():
            dict(q=step["q"].transpose(0, 1)), dict(q=step["q"][:, :5].contiguous()), dict(positions=step["positions"].long()),
            dict(block_tables=step["block_tables"][:1]), dict(query_start=step["query_start"][:2]), dict(context_lens=step["context_lens"].cpu()),
            dict(group_start=step["group_start"][:1]), dict(prefix_lens=step["prefix_lens"].float()), dict(max_query_len=-1), dict(max_prefix_len=-1),
-           dict(max_group_tokens=0), dict(softcap=-1.0), dict(softcap=float("nan")), dict(sink=torch.zeros(3, device="cuda")),
+           dict(max_group_tokens=0), dict(softcap=-1.0), dict(softcap=float("nan")), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(sink=torch.zeros(3, device="cuda")),
            dict(group_start=step["group_start"][:1], prefix_lens=step["prefix_lens"][:0])]
     for other in bad:
         with pytest.raises(KernelError):
