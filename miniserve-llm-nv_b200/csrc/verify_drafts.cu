@@ -11,6 +11,11 @@
 // Two kernels, both bound by the reads: of all rows of logits, then of one row of logits, draft probabilities and variates per request.  A
 // cluster of eight blocks works on a row: a block's eighth (76 KB of a vocabulary of 151,936) is read from memory once and stays in the
 // first-level cache for the passes that the filters take; counts, masses and candidates meet in distributed shared memory.
+//
+// The filters' borders are found in two passes: counts and masses in 2,048 bins of 1/64 of (max - x) / temperature (equal steps in the exponent spread the
+// entries; the bits of the numbers would put most into a few bins, whose atomics wait for one another), then the entries of the bin that holds the border,
+// ranked one by one.  Masses are sums of integers (units of 2^-44 of the largest weight at 151,936 entries), so that their order changes nothing.  Where
+// a bin holds more than the list takes (equal logits) or the border lies behind the bins, three rounds over the bits of the numbers find it.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -21,7 +26,9 @@ namespace verify {
 namespace cg = cooperative_groups;
 
 constexpr int kRanks = 8, kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048;              // of one round of a search over 32-bit keys: eleven, eleven and ten bits
+constexpr int kBins = 2048;              // also of one round of a search over 32-bit keys: eleven, eleven and ten bits
+constexpr float kBinsToOne = 64.f;
+constexpr int kListed = 1024;            // entries of a border's bin that are ranked one by one
 
 struct Record {  // one per state slot, as `sample` reads it
   float temperature;
@@ -34,7 +41,7 @@ struct Row {      // what the second kernel needs to know of a row
   float top, inverse;      // the largest logit, and 1 / the kept sum of e^((x - top) / temperature)
   unsigned thr;            // kept: order_key > thr, or equal to it and an index below bound
   int bound;
-  int best;                // argmax
+  int best;                // argmax (temperature 0)
   int passes;              // its draft passes
   int reserved[2];
 };
@@ -43,6 +50,7 @@ __device__ __forceinline__ unsigned order_key(float f) {
   const unsigned u = __float_as_uint(f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float number_of(unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); }
 
 struct Best {
   float value;
@@ -56,6 +64,13 @@ __device__ __forceinline__ Best better(Best a, Best b) {
 __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.f : -INFINITY; }
 // (x - top) / temperature, 0 at x = top also where both are infinite.
 __device__ __forceinline__ float exponent(float x, float top, float temperature) { return x == top ? 0.f : (x - top) / temperature; }
+// e^((x - top) / temperature) with per = log2 e / temperature: of the sums and the quotients, where a weight that is off by 2^-21 of itself (e^-10 and
+// below; the large ones are off by 2^-22) changes nothing but a choice between two quotients that near.
+__device__ __forceinline__ float quick_weight(float x, float top, float per) {
+  float w;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(x == top ? 0.f : (x - top) * per));
+  return w;
+}
 
 // This block's part of a row, in index order over the ranks; the parts start at 16-byte boundaries.
 struct Part {
@@ -67,46 +82,72 @@ struct Part {
     begin = rank == 0 ? 0 : min(v, rank * per + lead);
     end = rank == kRanks - 1 ? v : min(v, (rank + 1) * per + lead);
   }
-  template <typename F> __device__ __forceinline__ void each(F f) const {
+  // f(x, first): sixteen entries; number 4 j + e has the index first + 4 kThreads j + e, and is -inf where there is none.
+  template <typename F> __device__ __forceinline__ void sixteen(F f) const {
     const int lead = (int)((16 - (reinterpret_cast<uintptr_t>(row + begin) & 15)) & 15) / 4;
     const int first = min(end, begin + lead), quads = (end - first) / 4;
-    if (begin + (int)threadIdx.x < first) f(begin + (int)threadIdx.x, clean(row[begin + threadIdx.x]));
     const float4* wide = reinterpret_cast<const float4*>(row + first);
     for (int g = threadIdx.x; g < quads; g += 4 * kThreads) {
-      float4 v[4];
+      float x[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (g + j * kThreads < quads) v[j] = wide[g + j * kThreads];
+      for (int j = 0; j < 4; ++j) {
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (g + j * kThreads < quads) v = wide[g + j * kThreads];
+        x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (g + j * kThreads < quads) {
-          const int i = first + 4 * (g + j * kThreads);
-          f(i, clean(v[j].x)), f(i + 1, clean(v[j].y)), f(i + 2, clean(v[j].z)), f(i + 3, clean(v[j].w));
-        }
+      for (int j = 0; j < 16; ++j) x[j] = clean(x[j]);
+      f(x, first + 4 * g);
     }
-    const int tail = first + 4 * quads + (int)threadIdx.x;
-    if (tail < end) f(tail, clean(row[tail]));
+    // the ragged ends: up to three entries before the first boundary and behind the last
+    const int ends = first - begin + (end - first - 4 * quads);
+    if ((int)threadIdx.x < ends) {
+      const int i = (int)threadIdx.x < first - begin ? begin + (int)threadIdx.x : first + 4 * quads + (int)threadIdx.x - (first - begin);
+      float x[16];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) x[j] = -INFINITY;
+      x[0] = clean(row[i]);
+      f(x, i);
+    }
+  }
+  template <typename F> __device__ __forceinline__ void each(F f) const {      // f(index, x) of every entry that is not masked
+    sixteen([&](const float (&x)[16], int first) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (x[j] > -INFINITY) f(first + (j / 4) * 4 * kThreads + j % 4, x[j]);
+    });
   }
 };
 
-struct Shared {
-  unsigned long long bins[2][kBins];       // this block's, in one of two buffers in turn: a rank may still read the last round's
-  unsigned long long scan[kWarps];
-  double sums[2][kRanks];
+struct Entry {
+  float x;
+  int index;
+  unsigned long long mass;
+};
+
+struct Joined {
   Best bests[2][kRanks];
-  float tops[2][kRanks];
-  int counts[2][kRanks];
-  float warp_float[kWarps];
-  double warp_double[kWarps];
   Best warp_best[kWarps];
+};
+
+struct Shared : Joined {
+  unsigned long long mass[kBins];
+  unsigned count[kBins];
+  Entry list[kListed];
+  int listed;
+  unsigned long long scan[kWarps];
+  double sums[kRanks];
+  int counts[kRanks];
+  double warp_double[kWarps];
   int warp_int[kWarps];
-  int found;
-  unsigned long long above;
+  int found, bin, bound;
+  unsigned thr;
+  unsigned long long above, kept;
 };
 
 // Values of all threads of the cluster, joined in a fixed order: every rank writes its block's into slot `rank` of every rank's array.  `turn`
-// alternates, so that no rank's next value overtakes a slower rank's reads.
-__device__ Best cluster_best(Shared& s, cg::cluster_group& cluster, int rank, Best v, int turn) {
+// alternates where it is called twice, so that no rank's next value overtakes a slower rank's reads.
+__device__ Best cluster_best(Joined& s, cg::cluster_group& cluster, int rank, Best v, int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -128,7 +169,7 @@ __device__ Best cluster_best(Shared& s, cg::cluster_group& cluster, int rank, Be
   return b;
 }
 
-__device__ double cluster_sum(Shared& s, cg::cluster_group& cluster, int rank, double v, int turn) {
+__device__ double cluster_sum(Shared& s, cg::cluster_group& cluster, int rank, double v) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -137,27 +178,24 @@ __device__ double cluster_sum(Shared& s, cg::cluster_group& cluster, int rank, d
   if (threadIdx.x < kRanks) {
     double b = 0.0;
     for (int w = 0; w < kWarps; ++w) b += s.warp_double[w];
-    cluster.map_shared_rank(&s, threadIdx.x)->sums[turn][rank] = b;
+    cluster.map_shared_rank(&s, threadIdx.x)->sums[rank] = b;
   }
   cluster.sync();
   double b = 0.0;
-  for (int r = 0; r < kRanks; ++r) b += s.sums[turn][r];
+  for (int r = 0; r < kRanks; ++r) b += s.sums[r];
   return b;
 }
 
-// One round of a search from the largest key down: with this round's bins filled on every rank, the highest bin at which the sum over it and
-// all higher ones exceeds `limit` (bin 0 where none does); `above`: the sum over the higher ones.
-__device__ int find_bin(Shared& s, cg::cluster_group& cluster, int buffer, unsigned long long limit, unsigned long long& above) {
-  cluster.sync();
+// Over this block's bins from the first on: the first at which the running sum exceeds `limit` (kBins where none does); `above`: the sum before it.
+template <typename T>
+__device__ int first_over(Shared& s, const T* bins, unsigned long long limit, unsigned long long& above) {
   constexpr int kEach = kBins / kThreads;
-  unsigned long long mine[kEach] = {};
-  // thread t holds the bins kBins - 1 - (t kEach + j): the largest keys first
+  unsigned long long mine[kEach], sum = 0;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    for (int r = 0; r < kRanks; ++r) mine[j] += cluster.map_shared_rank(&s, r)->bins[buffer][kBins - 1 - (threadIdx.x * kEach + j)];
-  unsigned long long sum = 0;
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) sum += mine[j];
+  for (int j = 0; j < kEach; ++j) {
+    mine[j] = bins[threadIdx.x * kEach + j];
+    sum += mine[j];
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long before = sum;
 #pragma unroll
@@ -165,26 +203,36 @@ __device__ int find_bin(Shared& s, cg::cluster_group& cluster, int buffer, unsig
     const unsigned long long other = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += other;
   }
-  if (threadIdx.x == 0) s.found = -1;
+  __syncthreads();
   if (lane == 31) s.scan[warp] = before;
+  if (threadIdx.x == 0) s.found = kBins;
   __syncthreads();
   before -= sum;
   for (int w = 0; w < warp; ++w) before += s.scan[w];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     if (before <= limit && before + mine[j] > limit) {          // true at one bin at most
-      s.found = kBins - 1 - (threadIdx.x * kEach + j);
+      s.found = (int)threadIdx.x * kEach + j;
       s.above = before;
     }
     before += mine[j];
   }
-  if (threadIdx.x == kThreads - 1 && before <= limit) {
-    s.found = 0;
-    s.above = before - mine[kEach - 1];
-  }
+  if (threadIdx.x == kThreads - 1 && before <= limit) s.above = before;
   __syncthreads();
   above = s.above;
   return s.found;
+}
+
+// All ranks' bins added up in rank 0's, which calls this.
+template <typename T>
+__device__ void gather_bins(cg::cluster_group& cluster, T* bins) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    T sum = bins[i];
+#pragma unroll
+    for (int r = 1; r < kRanks; ++r) sum += *cluster.map_shared_rank(bins + i, r);
+    bins[i] = sum;
+  }
+  __syncthreads();
 }
 
 // The largest index bound with at most `need` entries below it for which `is` holds, over the whole row: ranks hold its parts in order.
@@ -201,16 +249,16 @@ __device__ int index_bound(Shared& s, cg::cluster_group& cluster, int rank, cons
   if (threadIdx.x < kRanks) {
     int all = 0;
     for (int w = 0; w < kWarps; ++w) all += s.warp_int[w];
-    cluster.map_shared_rank(&s, threadIdx.x)->counts[0][rank] = all;
+    cluster.map_shared_rank(&s, threadIdx.x)->counts[rank] = all;
   }
   cluster.sync();
   int before = 0, owner = kRanks - 1;
   for (int r = 0; r < kRanks; ++r) {
-    if (before + s.counts[0][r] > need) {
+    if (before + s.counts[r] > need) {
       owner = r;
       break;
     }
-    if (r + 1 < kRanks) before += s.counts[0][r];
+    if (r + 1 < kRanks) before += s.counts[r];
   }
   if (rank == owner) {
     // the entry number `need` (from 0) of those for which `is` holds is the first that is not taken
@@ -229,10 +277,10 @@ __device__ int index_bound(Shared& s, cg::cluster_group& cluster, int rank, cons
       __syncthreads();
       if (before > need) break;
     }
-    if (threadIdx.x < kRanks) cluster.map_shared_rank(&s, threadIdx.x)->counts[1][0] = s.found;
+    if (threadIdx.x < kRanks) cluster.map_shared_rank(&s, threadIdx.x)->bound = s.found;
   }
   cluster.sync();
-  return s.counts[1][0];
+  return s.bound;
 }
 
 __device__ __forceinline__ int request_of(const int* draft_start, int requests, int row) {
@@ -244,8 +292,248 @@ __device__ __forceinline__ int request_of(const int* draft_start, int requests, 
   return low;
 }
 
+// A row's weights as sums of integers: units of 2^-shift of the largest.  Of the entries near the largest, which make up most of a mass, the exponential in
+// float64: which entry a border falls on then does not hang on the rounding of the largest terms.
+struct Weights {
+  float top, temperature, to_bin;
+  double unit;
+  __device__ Weights(float t, float heat, int shift) : top(t), temperature(heat), to_bin(kBinsToOne / heat), unit((double)(1ull << shift)) {}
+  __device__ __forceinline__ unsigned long long of(float x) const {
+    const float e = exponent(x, top, temperature);
+    if (e > -7.f) return (unsigned long long)__double2ll_rn(exp(x == top ? 0.0 : ((double)x - (double)top) / (double)temperature) * unit);
+    return (unsigned long long)__float2ll_rn(expf(e) * (float)unit);
+  }
+  // (entries of one bin have a higher number than those of the bins before it are smaller than they; behind the last bin: kBins)
+  __device__ __forceinline__ int bin(float x) const {
+    const float t = x == top ? 0.f : (top - x) * to_bin;
+    return t < (float)kBins ? (int)t : kBins;
+  }
+};
+
+// The kept set of a row with filters by two passes; false on every rank where the border's bin is too full or the border lies behind the bins.  On
+// rank 0 row.thr, row.bound and `total`, the kept mass, are set.
+__device__ bool filter_by_bins(Shared& s, cg::cluster_group& cluster, int rank, const Part& part, const Weights& weights, const Record& rec, bool top_k,
+                               bool top_p, Row& row, unsigned long long& total) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+  if (threadIdx.x == 0) s.listed = 0;
+  __syncthreads();
+  part.each([&](int, float x) {
+    const int bin = weights.bin(x);
+    if (bin >= kBins) return;                   // (less than e^-32 of the largest: no mass)
+    const unsigned long long w = weights.of(x);
+    if (w != 0) atomicAdd(&s.mass[bin], w);
+    if (top_k) atomicAdd(&s.count[bin], 1u);
+  });
+  cluster.sync();
+  // rank 0 alone searches; `bin` says which bin's entries all ranks are to send it: -1 none, -2 give up
+  unsigned long long limit = 0, above = 0, before = 0;       // of the mass
+  int need = 0;                                               // top_k: how many of the bin's entries stay
+  if (rank == 0) {
+    gather_bins(cluster, s.mass);
+    if (top_k) gather_bins(cluster, s.count);
+    int bin;
+    if (top_k) {
+      bin = first_over(s, s.count, (unsigned long long)rec.top_k - 1, before);
+      need = rec.top_k - (int)before;
+      if (bin == kBins) bin = -2;
+    } else {
+      first_over(s, s.mass, ~0ull - 1, total);                // (all of it)
+      limit = (unsigned long long)floor((double)rec.top_p * (double)total);
+      bin = first_over(s, s.mass, limit, above);
+      if (bin == kBins) bin = -2;
+    }
+    if (threadIdx.x < kRanks) cluster.map_shared_rank(&s, threadIdx.x)->bin = bin;
+  }
+#pragma unroll 1
+  for (int round = 0; round < 2; ++round) {
+    cluster.sync();
+    const int bin = s.bin;
+    if (bin < 0) break;
+    Shared* first = cluster.map_shared_rank(&s, 0);
+    part.each([&](int i, float x) {
+      if (weights.bin(x) != bin) return;
+      const int at = atomicAdd(&first->listed, 1);
+      if (at < kListed) first->list[at] = Entry{x, i, weights.of(x)};
+    });
+    cluster.sync();
+    if (rank == 0) {
+      const int listed = s.listed;
+      int next = listed > kListed ? -2 : -1;
+      if (next == -1) {
+        const bool by_count = top_k && round == 0;
+        if (by_count) {
+          // the mass before this bin, then that of the entries that stay
+          unsigned long long part_mass = 0;
+          for (int i = threadIdx.x; i < bin; i += kThreads) part_mass += s.mass[i];
+          if (threadIdx.x == 0) s.above = 0, s.kept = 0;
+          __syncthreads();
+          if (part_mass != 0) atomicAdd(&s.above, part_mass);
+          __syncthreads();
+          above = s.above;
+        }
+        // an entry's place in the bin, and the mass of those before it; of those that stay the last one is the border
+        auto solve = [&](bool count, bool mass, int most) {
+          __syncthreads();
+          if (threadIdx.x == 0) s.found = -1, s.kept = 0;
+          __syncthreads();
+          constexpr int kEach = kListed / kThreads;
+          int place[kEach];
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) {
+            const int a = (int)threadIdx.x + j * kThreads;
+            place[j] = -2;
+            if (a >= listed) continue;
+            const Entry mine = s.list[a];
+            unsigned long long sum = 0;
+            int ahead = 0;
+            for (int c = 0; c < listed; ++c) {
+              const Entry other = s.list[c];
+              if (other.x > mine.x || (other.x == mine.x && other.index < mine.index)) ++ahead, sum += other.mass;
+            }
+            place[j] = ahead;
+            if ((!count || ahead < most) && (!mass || above + sum <= limit)) {
+              atomicAdd(&s.kept, mine.mass);
+              atomicMax(&s.found, ahead);
+            }
+          }
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < kEach; ++j)
+            if (place[j] == s.found) {
+              const Entry mine = s.list[threadIdx.x + j * kThreads];
+              s.thr = order_key(mine.x), s.bound = mine.index + 1;
+            }
+          __syncthreads();
+          total = above + s.kept;
+        };
+        if (by_count) {
+          solve(true, false, need);
+          if (top_p) {
+            limit = (unsigned long long)floor((double)rec.top_p * (double)total);
+            if (limit >= above) {
+              solve(true, true, need);              // the nucleus ends in this bin
+            } else {
+              unsigned long long in_front;
+              next = first_over(s, s.mass, limit, in_front);
+              above = in_front;
+            }
+          }
+        } else {
+          solve(false, true, 0);
+        }
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) s.listed = 0;
+      if (threadIdx.x < kRanks) cluster.map_shared_rank(&s, threadIdx.x)->bin = next;
+      row.thr = s.thr, row.bound = s.bound;
+    }
+  }
+  cluster.sync();
+  return s.bin != -2;
+}
+
+// The same by three rounds over the bits of the numbers, the largest first, which takes any row.
+__device__ void filter_by_bits(Shared& s, cg::cluster_group& cluster, int rank, const Part& part, const Weights& weights, const Record& rec, bool top_k,
+                               bool top_p, Row& row, unsigned long long& total) {
+  row.thr = 0, row.bound = part.vocab;
+  unsigned prefix = 0;
+  int most = 0;
+  if (top_k) {
+    unsigned long long rest = (unsigned long long)rec.top_k - 1;
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+      const int low = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+      for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+      __syncthreads();
+      part.each([&](int, float x) {
+        const unsigned key = order_key(x);
+        if (round == 0 || (key >> (low + bits)) == prefix) atomicAdd(&s.count[kBins - 1 - ((key >> low) & ((1u << bits) - 1u))], 1u);
+      });
+      cluster.sync();
+      if (rank == 0) {
+        gather_bins(cluster, s.count);
+        unsigned long long before;
+        const int bin = first_over(s, s.count, rest, before);
+        rest -= before;
+        if (threadIdx.x < kRanks) {
+          Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
+          other->bin = bin, other->bound = (int)rest + 1;
+        }
+      }
+      cluster.sync();
+      if (s.bin == kBins) break;                     // fewer entries than top_k: all stay
+      prefix = (prefix << bits) | (unsigned)(kBins - 1 - s.bin);
+      most = s.bound;
+    }
+    if (s.bin != kBins) {
+      const unsigned thr = prefix;
+      row.thr = thr;
+      row.bound = index_bound(s, cluster, rank, part, most, [&](int, float x) { return order_key(x) == thr; });
+    }
+  }
+  const unsigned thr_k = row.thr;
+  const int bound_k = row.bound;
+  auto kept = [&](unsigned key, int i) { return key > thr_k || (key == thr_k && i < bound_k); };
+  if (!top_p) {
+    double sum = 0.0;
+    part.each([&](int i, float x) {
+      if (kept(order_key(x), i)) sum += (double)weights.of(x);
+    });
+    total = (unsigned long long)cluster_sum(s, cluster, rank, sum);
+    return;
+  }
+  unsigned long long limit = 0, above = 0;           // (rank 0's)
+  prefix = 0;
+#pragma unroll 1
+  for (int round = 0; round < 3; ++round) {
+    const int low = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+    cluster.sync();                                  // (rank 0 may still read)
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
+    __syncthreads();
+    part.each([&](int i, float x) {
+      const unsigned key = order_key(x);
+      if ((round == 0 || (key >> (low + bits)) == prefix) && kept(key, i)) {
+        const unsigned long long w = weights.of(x);
+        if (w != 0) atomicAdd(&s.mass[kBins - 1 - ((key >> low) & ((1u << bits) - 1u))], w);
+      }
+    });
+    cluster.sync();
+    if (rank == 0) {
+      gather_bins(cluster, s.mass);
+      if (round == 0) {
+        first_over(s, s.mass, ~0ull - 1, total);
+        limit = (unsigned long long)floor((double)rec.top_p * (double)total);
+      }
+      unsigned long long before;
+      const int bin = min(first_over(s, s.mass, limit - above, before), kBins - 1);
+      above += before;
+      if (round == 2) {
+        // of the equal entries at the border those stay whose mass before is at most the limit
+        const unsigned long long each = weights.of(number_of((prefix << bits) | (unsigned)(kBins - 1 - bin)));
+        const unsigned long long room = each > 0 ? (limit - above) / each + 1 : 1, there = each > 0 ? s.mass[bin] / each : 0;
+        const unsigned long long stay = room < there ? room : there;
+        total = above + stay * each;
+        most = room < (unsigned long long)part.vocab ? (int)room : part.vocab;
+      }
+      if (threadIdx.x < kRanks) {
+        Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
+        other->bin = bin, other->bound = most;
+      }
+    }
+    cluster.sync();
+    prefix = (prefix << bits) | (unsigned)(kBins - 1 - s.bin);
+    most = s.bound;
+  }
+  if (prefix >= thr_k) {
+    const unsigned thr = prefix;
+    const int outer = thr == thr_k ? bound_k : part.vocab;
+    row.thr = thr;
+    row.bound = min(outer, index_bound(s, cluster, rank, part, most, [&](int i, float x) { return order_key(x) == thr && i < outer; }));
+  }
+}
+
 // Cluster: a row of logits.
-__global__ void __cluster_dims__(kRanks, 1, 1) __launch_bounds__(kThreads)
+__global__ void __cluster_dims__(kRanks, 1, 1) __launch_bounds__(kThreads, 2)
 verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __restrict__ drafts, const int* __restrict__ draft_start, int requests,
                    int total, const float* __restrict__ uniforms, const float* __restrict__ draft_probs, const Record* __restrict__ records,
                    const int* __restrict__ slots, Row* __restrict__ out, float* __restrict__ target_probs, int shift) {
@@ -262,131 +550,63 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
   const bool greedy = !(rec.temperature > 0.f);
   const bool top_k = rec.top_k > 0 && rec.top_k < vocab, top_p = rec.top_p < 1.f;
   const Part part(logits + (size_t)r * vocab, vocab, rank);
-
-  Best best{-INFINITY, 0x7fffffff};
-  double sum = 0.0;
-  // without filters one pass gives the sum too: relative to the thread's own running maximum
-  const bool one_pass = !greedy && !top_k && !top_p;
-  float partial = 0.f;
-  part.each([&](int i, float x) {
-    if (x > best.value) {
-      if (one_pass && best.value > -INFINITY) partial *= expf(exponent(best.value, x, rec.temperature));
-      best = Best{x, i};
-    }
-    if (one_pass && x > -INFINITY) partial += expf(exponent(x, best.value, rec.temperature));
-  });
-  const float mine = best.value;
-  best = cluster_best(s, cluster, rank, best, 0);
-  const float top = best.value;
-  const bool nothing = top == -INFINITY;            // every entry is masked: no token has a probability
-  Row row{};
-  row.top = top;
-  row.best = best.index == 0x7fffffff ? 0 : best.index;
-  row.bound = vocab;
   const int token = drafted ? drafts[draft] : 0;
   const bool known = drafted && token >= 0 && token < vocab;
+  Row row{};
+  row.bound = vocab;
   float p = 0.f;
+  Best best{-INFINITY, 0x7fffffff};
   if (greedy) {
-    p = known && !nothing && token == row.best ? 1.f : 0.f;
+    part.sixteen([&](const float (&x)[16], int first) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (x[j] > -INFINITY) best = better(best, Best{x[j], first + (j / 4) * 4 * kThreads + j % 4});
+    });
+    best = cluster_best(s, cluster, rank, best, 0);
+    row.best = best.index == 0x7fffffff ? 0 : best.index;
+    p = known && best.index == token ? 1.f : 0.f;
     row.passes = p > 0.f;
-  } else if (!nothing) {
-    const float temperature = rec.temperature;
-    // of the entries near the largest, which make up most of a mass, the exponential in float64: which entry a border falls on then does not hang
-    // on the rounding of the largest terms
-    auto weight = [&](float x) {
-      const float e = exponent(x, top, temperature);
-      return e > -7.f ? exp(x == top ? 0.0 : ((double)x - (double)top) / (double)temperature) : (double)expf(e);
-    };
-    if (one_pass) {
-      sum = mine == -INFINITY ? 0.0 : (double)(partial * expf(exponent(mine, top, temperature)));
-      sum = cluster_sum(s, cluster, rank, sum, 0);
-    } else {
-      int buffer = 0;
-      auto clear = [&](int b) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[b][i] = 0;
-        __syncthreads();
-      };
-      if (top_k) {
-        unsigned prefix = 0;
-        unsigned long long rest = (unsigned long long)rec.top_k - 1, above = 0;
-#pragma unroll 1
-        for (int round = 0; round < 3; ++round) {
-          const int low = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
-          clear(buffer);
-          part.each([&](int, float x) {
-            const unsigned key = order_key(x);
-            if (round == 0 || (key >> (low + bits)) == prefix) atomicAdd(&s.bins[buffer][(key >> low) & ((1u << bits) - 1u)], 1ull);
-          });
-          const int bin = find_bin(s, cluster, buffer, rest, above);
-          rest -= above;
-          prefix = (prefix << bits) | (unsigned)bin;
-          buffer ^= 1;
-        }
-        row.thr = prefix;
-        // rest: how many of the entries equal to the threshold stand before the last kept one
-        const unsigned thr = row.thr;
-        row.bound = index_bound(s, cluster, rank, part, (int)rest + 1, [&](int, float x) { return order_key(x) == thr; });
+  } else {
+    // the largest, and without filters in the same pass the sum relative to this thread's running maximum
+    const bool one_pass = !top_k && !top_p;
+    const float per = 1.4426950408889634f / rec.temperature;
+    float partial = 0.f;
+    part.sixteen([&](const float (&x)[16], int) {
+      float m = x[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) m = fmaxf(m, x[j]);
+      if (m > best.value) {
+        if (one_pass && best.value > -INFINITY) partial *= quick_weight(best.value, m, per);
+        best.value = m;
       }
-      const unsigned thr_k = row.thr;
-      const int bound_k = row.bound;
-      auto kept = [&](unsigned key, int i) { return key > thr_k || (key == thr_k && i < bound_k); };
-      if (top_p) {
-        const double unit = (double)(1ull << shift);
-        auto fixed = [&](float x) { return (unsigned long long)__double2ll_rn(weight(x) * unit); };
-        double all = 0.0;
-        unsigned prefix = 0;
-        unsigned long long limit = 0, above = 0, so_far = 0;
-        {
-          double z = 0.0;
-          part.each([&](int i, float x) {
-            if (kept(order_key(x), i)) z += (double)fixed(x);
-          });
-          all = cluster_sum(s, cluster, rank, z, 0);
-        }
-        limit = (unsigned long long)floor((double)rec.top_p * all);
-#pragma unroll 1
-        for (int round = 0; round < 3; ++round) {
-          const int low = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
-          clear(buffer);
-          part.each([&](int i, float x) {
-            const unsigned key = order_key(x);
-            if ((round == 0 || (key >> (low + bits)) == prefix) && kept(key, i)) {
-              const unsigned long long w = fixed(x);
-              if (w != 0) atomicAdd(&s.bins[buffer][(key >> low) & ((1u << bits) - 1u)], w);
-            }
-          });
-          const int bin = find_bin(s, cluster, buffer, limit - so_far, above);
-          so_far += above;
-          prefix = (prefix << bits) | (unsigned)bin;
-          buffer ^= 1;
-        }
-        if (prefix >= thr_k) {
-          // of the entries equal to the threshold those stay whose mass before is at most the limit
-          const float x = __uint_as_float((prefix & 0x80000000u) ? (prefix & 0x7fffffffu) : ~prefix);
-          const unsigned long long each = fixed(x);
-          const unsigned long long room = each > 0 ? (limit - so_far) / each + 1 : 1;
-          const int most = room > (unsigned long long)vocab ? vocab : (int)room;
-          row.thr = prefix;
-          const int outer = prefix == thr_k ? bound_k : vocab;
-          const unsigned thr = prefix;
-          row.bound = min(outer, index_bound(s, cluster, rank, part, most, [&](int i, float v) { return order_key(v) == thr && i < outer; }));
-        }
+      if (one_pass && best.value > -INFINITY) {
+        float sum[4] = {};
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[j & 3] += quick_weight(x[j], best.value, per);
+        partial += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
-      const unsigned thr = row.thr;
-      const int bound = row.bound;
-      part.each([&](int i, float x) {
+    });
+    const float mine = best.value;
+    row.top = cluster_best(s, cluster, rank, best, 0).value;
+    if (row.top > -INFINITY) {                   // (else every entry is masked: no token has a probability)
+      double sum = 0.0;                          // (rank 0's)
+      if (one_pass) {
+        sum = cluster_sum(s, cluster, rank, mine == -INFINITY ? 0.0 : (double)(partial * quick_weight(mine, row.top, per)));
+      } else {
+        const Weights weights(row.top, rec.temperature, shift);
+        unsigned long long mass = 0;
+        if (!filter_by_bins(s, cluster, rank, part, weights, rec, top_k, top_p, row, mass))
+          filter_by_bits(s, cluster, rank, part, weights, rec, top_k, top_p, row, mass);
+        sum = (double)mass / weights.unit;
+      }
+      row.inverse = sum > 0.0 ? (float)(1.0 / sum) : 0.f;
+      if (known) {
+        const float x = clean(part.row[token]);
         const unsigned key = order_key(x);
-        if (key > thr || (key == thr && i < bound)) sum += weight(x);
-      });
-      sum = cluster_sum(s, cluster, rank, sum, 1);
-    }
-    row.inverse = sum > 0.0 ? (float)(1.0 / sum) : 0.f;
-    if (known) {
-      const float x = clean(part.row[token]);
-      const unsigned key = order_key(x);
-      if (x > -INFINITY && (key > row.thr || (key == row.thr && token < row.bound))) p = expf(exponent(x, top, temperature)) * row.inverse;
-      const float q = draft_probs != nullptr ? draft_probs[(size_t)draft * vocab + token] : 1.f;
-      row.passes = uniforms[draft] * q < p;
+        if (x > -INFINITY && (key > row.thr || (key == row.thr && token < row.bound))) p = expf(exponent(x, row.top, rec.temperature)) * row.inverse;
+        const float q = draft_probs != nullptr ? draft_probs[(size_t)draft * vocab + token] : 1.f;
+        row.passes = uniforms[draft] * q < p;
+      }
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
@@ -397,12 +617,12 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
 }
 
 // Cluster: a request.
-__global__ void __cluster_dims__(kRanks, 1, 1) __launch_bounds__(kThreads)
+__global__ void __cluster_dims__(kRanks, 1, 1) __launch_bounds__(kThreads, 2)
 verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __restrict__ drafts, const int* __restrict__ draft_start,
                      const float* __restrict__ noise, const float* __restrict__ draft_probs, const Record* __restrict__ records,
                      const int* __restrict__ slots, const Row* __restrict__ rows, int total, int* __restrict__ accepted,
                      int* __restrict__ next_token) {
-  __shared__ Shared s;
+  __shared__ Joined s;
   grid_dependency_wait();
   grid_dependency_launch();
   cg::cluster_group cluster = cg::this_cluster();
@@ -422,21 +642,52 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
   int chosen = row.best;
   if (!greedy && row.inverse > 0.f) {
     const bool rejected = passed < count;
-    const float* q = rejected && draft_probs != nullptr ? draft_probs + (size_t)(first + passed) * vocab : nullptr;
+    const float* x_row = logits + (size_t)r * vocab;
+    const float* q_row = rejected && draft_probs != nullptr ? draft_probs + (size_t)(first + passed) * vocab : nullptr;
+    const float* e_row = noise + (size_t)request * vocab;
     const int token = rejected ? drafts[first + passed] : -1;
-    const float* e = noise + (size_t)request * vocab;
-    const Part part(logits + (size_t)r * vocab, vocab, rank);
+    const float per = 1.4426950408889634f / rec.temperature;
+    // (rows of a vocabulary that is no multiple of four start at other boundaries each: numbers one by one)
+    const bool wide = vocab % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_probs) | reinterpret_cast<uintptr_t>(noise)) & 15) == 0;
+    const int quads = (vocab + 3) / 4, share = (quads + kRanks - 1) / kRanks, quad_end = min(quads, (rank + 1) * share);
     auto race = [&](bool residual) {
       Best best{-INFINITY, 0x7fffffff};
-      for (int i = part.begin + (int)threadIdx.x; i < part.end; i += kThreads) {
-        const float x = clean(part.row[i]);
-        const unsigned key = order_key(x);
-        if (!(x > -INFINITY) || !(key > row.thr || (key == row.thr && i < row.bound))) continue;
-        float left = expf(exponent(x, row.top, rec.temperature)) * row.inverse;
-        if (residual) left = q != nullptr ? left - q[i] : i == token ? 0.f : left;
-        if (!(left > 0.f)) continue;
-        const float value = left / e[i];
-        if (value > best.value) best = Best{value, i};
+      constexpr int kDeep = 2;
+      for (int g = rank * share + (int)threadIdx.x; g < quad_end; g += kDeep * kThreads) {
+        float x[kDeep][4], q[kDeep][4], e[kDeep][4];
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j) {
+          const int quad = g + j * kThreads, i = 4 * quad;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[j][c] = -INFINITY, q[j][c] = 0.f, e[j][c] = 1.f;
+          if (quad >= quad_end) continue;
+          if (wide) {
+            *reinterpret_cast<float4*>(x[j]) = *reinterpret_cast<const float4*>(x_row + i);
+            *reinterpret_cast<float4*>(e[j]) = *reinterpret_cast<const float4*>(e_row + i);
+            if (residual && q_row != nullptr) *reinterpret_cast<float4*>(q[j]) = *reinterpret_cast<const float4*>(q_row + i);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (i + c < vocab) {
+                x[j][c] = x_row[i + c], e[j][c] = e_row[i + c];
+                if (residual && q_row != nullptr) q[j][c] = q_row[i + c];
+              }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int i = 4 * (g + j * kThreads) + c;
+            const float v = clean(x[j][c]);
+            const unsigned key = order_key(v);
+            if (!(v > -INFINITY) || !(key > row.thr || (key == row.thr && i < row.bound))) continue;
+            float left = quick_weight(v, row.top, per) * row.inverse;
+            if (residual) left = q_row != nullptr ? left - q[j][c] : i == token ? 0.f : left;
+            if (!(left > 0.f)) continue;
+            const float value = left / e[j][c];
+            if (value > best.value || (value == best.value && i < best.index)) best = Best{value, i};
+          }
       }
       return best;
     };
