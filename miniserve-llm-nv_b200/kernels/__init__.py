@@ -129,14 +129,18 @@ def _want(tensor: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise KernelError(f"{name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}")
 
 
-def _want_here(**tensors: Optional[torch.Tensor]) -> None:
-    """All of them on the current device, whose streams the launches go to."""
-    current = torch.cuda.current_device()
-    for name, tensor in tensors.items():
-        if tensor is not None and tensor.is_cuda and tensor.get_device() != current:
-            raise KernelError(f"{name} lies on {tensor.device}, the current device is cuda:{current}")
-    if _device_index not in (None, current):
-        raise KernelError(f"the library's launches go to cuda:{_device_index}, the current device is cuda:{current}")
+def _want_all(checks: tuple) -> None:
+    """:func:`_want` of (tensor, name, dtype, shape) each (a tensor that is None is left out), all of them on the current device, whose streams the
+    launches go to."""
+    here = torch._C._cuda_getDevice()
+    if _device_index is not None and _device_index != here:
+        raise KernelError(f"the library's launches go to cuda:{_device_index}, the current device is cuda:{here}")
+    for tensor, name, dtype, shape in checks:
+        if tensor is None or (tensor.is_cuda and tensor.get_device() == here and tensor.is_contiguous() and (dtype is None or tensor.dtype is dtype)
+                              and (shape is None or tensor.shape == shape)):
+            continue
+        _want(tensor, name, dtype, shape)
+        raise KernelError(f"{name} lies on {tensor.device}, the current device is cuda:{here}")
 
 
 _i = int        # (arguments are converted by ctypes from the prototypes' types; these only coerce)
@@ -2451,31 +2455,23 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     (no window).  Upper bounds that shape the grids, which a captured launch keeps: ``max_query_len`` and ``max_group_tokens``, the
     most tokens of a request and of a group; ``max_prefix_len`` and ``max_suffix_len``, the most keys of a prefix and of a request behind it.
     A part's share of the keys depends on these bounds, and with it the rounding of the result."""
-    if q.dim() != 3 or k_pool.dim() != 4:
-        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)} are not [N, n_q, d] or the pool {tuple(k_pool.shape)} is not [pages, n_kv, page_size, d]")
+    if q.dim() != 3 or k_pool.dim() != 4 or block_tables.dim() != 2:
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)} are not [N, n_q, d], the pool {tuple(k_pool.shape)} is not [pages, n_kv, page_size, "
+                          f"d] or the tables {tuple(block_tables.shape)} are not [requests, width]")
     n, n_q, head_dim = q.shape
-    n_kv = k_pool.shape[1]
-    n_requests, n_groups = context_lens.numel(), prefix_lens.numel()
-    _want(q, "q")
-    _want(k_pool, "k_pool", q.dtype)
-    if k_pool.shape[3] != head_dim or n_kv < 1 or n_q % n_kv or k_pool.shape[2] < 1:
-        raise KernelError(f"pool shape {tuple(k_pool.shape)} is not [pages, a divisor of {n_q}, page_size, {head_dim}]")
-    _want(v_pool, "v_pool", q.dtype, k_pool.shape)
-    _want(out, "out", q.dtype, (n, n_q, head_dim))
-    if block_tables.dim() != 2 or block_tables.shape[0] != n_requests:
-        raise KernelError(f"block_tables {tuple(block_tables.shape)} for {n_requests} requests")
-    _want(block_tables, "block_tables", torch.int32)
-    _want(positions, "positions", torch.int32, (n,))
-    _want(query_start, "query_start", torch.int32, (n_requests + 1,))
-    _want(context_lens, "context_lens", torch.int32, (n_requests,))
-    _want(group_start, "group_start", torch.int32, (n_groups + 1,))
-    _want(prefix_lens, "prefix_lens", torch.int32, (n_groups,))
+    pages, n_kv, page_size, _ = k_pool.shape
+    n_requests, n_groups, dtype = context_lens.numel(), prefix_lens.numel(), q.dtype
     sink_scores = None
     if isinstance(sink, torch.Tensor):
-        _want(sink, "sink", torch.float32, (n_q,))
         sink, sink_scores = True, sink
-    _want_here(q=q, k_pool=k_pool, v_pool=v_pool, block_tables=block_tables, positions=positions, query_start=query_start,
-               context_lens=context_lens, group_start=group_start, prefix_lens=prefix_lens, sink=sink_scores, out=out)
+    _want_all(((q, "q", None, None), (k_pool, "k_pool", dtype, (pages, n_kv, page_size, head_dim)), (v_pool, "v_pool", dtype, k_pool.shape),
+               (out, "out", dtype, (n, n_q, head_dim)), (block_tables, "block_tables", torch.int32, (n_requests, block_tables.shape[1])),
+               (positions, "positions", torch.int32, (n,)), (query_start, "query_start", torch.int32, (n_requests + 1,)),
+               (context_lens, "context_lens", torch.int32, (n_requests,)), (group_start, "group_start", torch.int32, (n_groups + 1,)),
+               (prefix_lens, "prefix_lens", torch.int32, (n_groups,)), (sink_scores, "sink", torch.float32, (n_q,))))
+    code = _code(dtype)
+    if n_kv < 1 or n_q % n_kv or page_size < 1:
+        raise KernelError(f"pool shape {tuple(k_pool.shape)} is not [pages, a divisor of {n_q}, page_size, {head_dim}]")
     if not 1 <= head_dim <= MAX_HEAD_DIM:
         raise KernelError(f"head size {head_dim} is not in 1..{MAX_HEAD_DIM}")
     if min(max_query_len, max_group_tokens) < 0 or min(max_prefix_len, max_suffix_len) < 0 or max_group_tokens < max_query_len:
@@ -2490,20 +2486,20 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if n_requests == 0 or n_groups == 0:
         raise KernelError(f"{n} tokens of {n_requests} requests in {n_groups} groups")
     lib = library()
-    tensor = int(q.dtype is torch.bfloat16 and bool(_asked("ms_prefix_attention_on_tensor_cores", head_dim))
+    tensor = int(code == 1 and _asked("ms_prefix_attention_on_tensor_cores", head_dim) == 1
                  and (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16 == 0)
-    sizes = (tensor, head_dim, n_q, n_kv, k_pool.shape[2])
+    sizes = (tensor, head_dim, n_q, n_kv, page_size)
     prefix_parts = _asked("ms_prefix_attention_parts", 0, *sizes, n_groups, max_group_tokens, max_prefix_len) if max_prefix_len > 0 else 0
     own_parts = _asked("ms_prefix_attention_parts", 1, *sizes, n_requests, max_query_len, max_suffix_len)
     parts = prefix_parts + own_parts
-    part_o = torch.empty((n * n_q * parts, head_dim), dtype=torch.float32, device=q.device)
-    part_lse = torch.empty((n * n_q * parts,), dtype=torch.float32, device=q.device)
+    rows = n * n_q * parts
+    scratch = torch.empty(rows * (head_dim + 1), dtype=torch.float32, device=q.device)        # (outputs of the parts, then their log-sum-exps)
+    part_o = scratch.data_ptr()
     _check(lib.ms_prefix_attention(
-        _i(tensor), _ptr(q), _i(_code(q.dtype)), _ptr(k_pool), _ptr(v_pool), _i(k_pool.shape[0]), _ptr(block_tables), _i(block_tables.shape[1]),
-        _ptr(positions), _ptr(query_start), _ptr(context_lens), _ptr(group_start), _ptr(prefix_lens), _i(k_pool.shape[2]), _i(n_q), _i(n_kv),
-        _i(head_dim), _f(scale), _f(softcap or 0.0), _i(1 if sink else 0), _ptr(sink_scores), _ptr(out), _ptr(part_o), _ptr(part_lse),
-        _i(prefix_parts), _i(own_parts), _i(n_requests), _i(n_groups), _i(n), _i(max_query_len), _i(max_group_tokens),
-        _ptr(device_error_flag(q.device)), _stream()))
+        tensor, q.data_ptr(), code, k_pool.data_ptr(), v_pool.data_ptr(), pages, block_tables.data_ptr(), block_tables.shape[1],
+        positions.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(), group_start.data_ptr(), prefix_lens.data_ptr(), page_size, n_q, n_kv,
+        head_dim, _f(scale), _f(softcap or 0.0), 1 if sink else 0, _ptr(sink_scores), out.data_ptr(), part_o, part_o + 4 * rows * head_dim,
+        prefix_parts, own_parts, n_requests, n_groups, n, _i(max_query_len), _i(max_group_tokens), device_error_flag(q.device).data_ptr(), _stream()))
 
 
 MAX_COPIED_POOLS = 8
@@ -2521,19 +2517,19 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], sources: Sequ
         raise KernelError(f"copy_pages: {len(pools)} pools in one call (1..{MAX_COPIED_POOLS})")
     if isinstance(sources, torch.Tensor) or isinstance(destinations, torch.Tensor):
         raise KernelError("copy_pages: page numbers are the host's (a list), not a tensor")
+    _want_all([(pool, "a pool", None, None) for pool in pools])
+    pages = pools[0].shape[1] if pools[0].dim() > 1 else 0
     described = array.array("q")
-    for index, pool in enumerate(pools):
-        name = f"pools[{index}]"
-        _want(pool, name)
-        _want_here(**{name: pool})
-        if pool.dim() < 3 or pool.shape[1] != pools[0].shape[1] or pool.numel() == 0:
-            raise KernelError(f"{name} {tuple(pool.shape)} is not [runs, {pools[0].shape[1]} pages, ...]")
-        described.extend((pool.data_ptr(), pool.shape[0], pool.shape[1], pool.stride(1) * pool.element_size()))
+    for pool in pools:
+        shape = pool.shape
+        if len(shape) < 3 or shape[1] != pages or pool.numel() == 0:
+            raise KernelError(f"a pool {tuple(shape)} is not [runs, {pages} pages, ...]")
+        described.extend((pool.data_ptr(), shape[0], pages, pool.stride(1) * pool.element_size()))
     try:
         source, destination = array.array("i", sources), array.array("i", destinations)
     except (TypeError, OverflowError) as error:
         raise KernelError(f"copy_pages: page numbers are integers: {error}") from None
-    n, pages = len(source), pools[0].shape[1]
+    n = len(source)
     if len(destination) != n:
         raise KernelError(f"copy_pages: {n} sources for {len(destination)} destinations")
     if n == 0:
@@ -2572,30 +2568,19 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, draft_start: torch
         raise KernelError(f"verify_drafts: logits {tuple(logits.shape)} are not [rows, vocabulary]")
     rows, vocab = logits.shape
     total, requests = drafts.numel(), accepted.numel()
-    _want(logits, "logits", torch.float32)
     if rows != total + requests or (rows and vocab < 1):
         raise KernelError(f"verify_drafts: {rows} rows of {vocab} logits for {total} drafts of {requests} requests")
-    _want(drafts, "drafts", torch.int32, (total,))
-    _want(draft_start, "draft_start", torch.int32, (requests + 1,))
-    _want(accepted, "accepted", torch.int32, (requests,))
-    _want(next_token, "next_token", torch.int32, (requests,))
-    if draft_probs is not None:
-        _want(draft_probs, "draft_probs", torch.float32, (total, vocab))
-    if target_probs is not None:
-        _want(target_probs, "target_probs", torch.float32, (total,))
     if records is not None:
-        _want(records, "records", torch.int32)
         if records.dim() != 2 or records.shape[1] != SAMPLING_RECORD_WORDS:
             raise KernelError(f"records must be [slots, {SAMPLING_RECORD_WORDS}] int32")
         if slot_of_request is None or uniforms is None or noise is None:
             raise KernelError("verify_drafts: sampling records need slot_of_request, uniforms and noise")
-        _want(slot_of_request, "slot_of_request", torch.int32, (requests,))
-    if uniforms is not None:
-        _want(uniforms, "uniforms", torch.float32, (total,))
-    if noise is not None:
-        _want(noise, "noise", torch.float32, (requests, vocab))
-    _want_here(logits=logits, drafts=drafts, draft_start=draft_start, uniforms=uniforms, noise=noise, accepted=accepted, next_token=next_token,
-               draft_probs=draft_probs, records=records, slot_of_request=slot_of_request, target_probs=target_probs)
+    _want_all(((logits, "logits", torch.float32, None), (drafts, "drafts", torch.int32, (total,)),
+               (draft_start, "draft_start", torch.int32, (requests + 1,)), (accepted, "accepted", torch.int32, (requests,)),
+               (next_token, "next_token", torch.int32, (requests,)), (draft_probs, "draft_probs", torch.float32, (total, vocab)),
+               (target_probs, "target_probs", torch.float32, (total,)), (records, "records", torch.int32, None),
+               (slot_of_request if records is not None else None, "slot_of_request", torch.int32, (requests,)),
+               (uniforms, "uniforms", torch.float32, (total,)), (noise, "noise", torch.float32, (requests, vocab))))
     if requests == 0:
         return
     scratch = torch.empty(rows * _asked("ms_verify_row_bytes"), dtype=torch.uint8, device=logits.device)
