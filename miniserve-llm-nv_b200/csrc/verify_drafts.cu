@@ -916,7 +916,9 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
     // (rows of a vocabulary that is no multiple of four start at other boundaries each: numbers one by one)
     const bool wide = vocab % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_probs) | reinterpret_cast<uintptr_t>(noise)) & 15) == 0;
     const int quads = (vocab + 3) / 4, share = (quads + ranks - 1) / ranks, quad_end = min(quads, (rank + 1) * share);
+    const float border = row.thr == 0 ? -INFINITY : number_of(row.thr);
     auto race = [&](bool residual) {
+      const int out_of = residual && q_row == nullptr ? token : -1;          // (a draft that was not drawn: its own token has nothing left)
       Best best{-INFINITY, 0x7fffffff};
       constexpr int kDeep = 2;
       for (int g = rank * share + (int)threadIdx.x; g < quad_end; g += kDeep * kThreads) {
@@ -944,15 +946,12 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
         for (int j = 0; j < kDeep; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
+            // (indices grow along this thread's way, so that the first of equal ones stays; NaN is no candidate)
             const int i = 4 * (g + j * kThreads) + c;
-            const float v = clean(x[j][c]);
-            const unsigned key = order_key(v);
-            if (!(v > -INFINITY) || !(key > row.thr || (key == row.thr && i < row.bound))) continue;
-            float left = quick_weight(v, row.top, per) * row.inverse;
-            if (residual) left = q_row != nullptr ? left - q[j][c] : i == token ? 0.f : left;
-            if (!(left > 0.f)) continue;
-            const float value = left / e[j][c];
-            if (value > best.value || (value == best.value && i < best.index)) best = Best{value, i};
+            const float v = x[j][c];
+            const bool kept = v > border || (v == border && i < row.bound);
+            const float left = quick_weight(v, row.top, per) * row.inverse - q[j][c], value = __fdividef(left, e[j][c]);
+            if (kept && left > 0.f && i != out_of && value > best.value) best = Best{value, i};
           }
       }
       return best;
@@ -977,17 +976,17 @@ using namespace ms;
 namespace ms {
 namespace verify {
 
-// Blocks to a row: eight for few rows, whose latency counts; fewer for many, so that all rows' blocks fit on the multiprocessors at once, two to each, and
-// meet less often (272 rows of 151,936 with filters: eight NN us, one NN us).
-static int ranks_for(int rows) {
-  int ranks = kMostRanks;
-  while (ranks > 1 && (long long)rows * ranks > 256) ranks /= 2;
-  return ranks;
+// Blocks to a row: many for few rows, whose latency counts, and fewer for more, so that no more clusters are asked for than find room at once (two blocks a
+// multiprocessor, a cluster's within one of the GPU's parts; 36 rows of 32,011 with filters: eight blocks each 52 us, four 27).  Rows of a
+// large vocabulary keep two, which even out what the filters of different rows take (272 rows of 151,936: one each 199 us, two 177).
+static int ranks_for(int rows, int vocab) {
+  if (rows <= 32) return kMostRanks;
+  if (rows <= 64) return 4;
+  return rows <= 148 || vocab >= 32768 ? 2 : 1;
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(void (*kernel)(Params...), int rows, size_t smem, cudaStream_t stream, Args&&... args) {
-  const int ranks = ranks_for(rows);
+cudaError_t launch_clusters(void (*kernel)(Params...), int rows, int ranks, size_t smem, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(rows * ranks));
   config.blockDim = dim3(kThreads);
@@ -1027,10 +1026,10 @@ MS_EXPORT int ms_verify_drafts(const float* logits, int vocab, const int* drafts
   while (shift > 0 && ((long long)vocab >> (62 - shift)) != 0) --shift;
   cudaError_t e = allow_shared(verify_rows_kernel, sizeof(Shared));
   if (e == cudaSuccess)
-    e = launch_clusters(verify_rows_kernel, n_drafts + requests, sizeof(Shared), stream, logits, vocab, drafts, draft_start, requests, n_drafts, uniforms,
+    e = launch_clusters(verify_rows_kernel, n_drafts + requests, ranks_for(n_drafts + requests, vocab), sizeof(Shared), stream, logits, vocab, drafts, draft_start, requests, n_drafts, uniforms,
                                   draft_probs, (const Record*)records, slot_of_request, (Row*)scratch, target_probs, shift);
   if (e == cudaSuccess)
-    e = launch_clusters(verify_choose_kernel, requests, 0, stream, logits, vocab, drafts, draft_start, noise, draft_probs, (const Record*)records,
+    e = launch_clusters(verify_choose_kernel, requests, ranks_for(requests, vocab), 0, stream, logits, vocab, drafts, draft_start, noise, draft_probs, (const Record*)records,
                         slot_of_request, (const Row*)scratch, n_drafts, accepted, next_token);
   if (e != cudaSuccess) cudaGetLastError();
   MS_REQUIRE(e == cudaSuccess, "verify_drafts: launch failed: %s", cudaGetErrorString(e));
