@@ -293,11 +293,11 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
     }
     return parts;
   }
-  // small blocks: so many that they fill the multiprocessors, a part keeping two tiles or more
-  const bool few = rows <= 16;
-  const long long base = (long long)units * n_kv * (tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
-  const long long slots = 148 * (tensor ? (few ? 5 : 2) : 4);
-  const int keep = tensor ? (few ? 64 : 128) : 128;
+  // small blocks: so many that they fill the multiprocessors, a part keeping some tiles
+  const bool few = rows <= 16, ring = tensor && own && prefix::own_tma_takes(d, page_size, 0);
+  const long long base = (long long)units * n_kv * (ring ? (rows <= 32 ? 1 : (rows + 63) / 64) : tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
+  const long long slots = 148 * (ring ? (few ? 12 : 6) : tensor ? (few ? 5 : 2) : 4);
+  const int keep = ring ? 128 : tensor ? (few ? 64 : 128) : 128;
   parts = (int)((slots + base - 1) / base);
   if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;
   if (parts > most) parts = most;
@@ -335,7 +335,10 @@ MS_EXPORT int ms_prefix_attention(int tensor, const void* q, int dtype, const vo
       code = launch_prefix_tcgen05(q, k_pool, v_pool, n_pages, b, parts, d, n_tokens, max_group_tokens, scale, softcap, error_flag, stream);
     else if (shared)
       code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_group_tokens, scale, softcap, false, false, stream);
-    if (code == 0) code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_query_len, scale, softcap, true, shared, stream);
+    if (code == 0 && own_tma_takes(d, page_size, (long long)n_pages * n_kv * page_size))
+      code = launch_own_tma(q, k_pool, v_pool, n_pages, b, parts, d, max_query_len, scale, softcap, shared, error_flag, stream);
+    else if (code == 0)
+      code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_query_len, scale, softcap, true, shared, stream);
     if (code != 0) return code;
     if (d <= 64) return launch_join<__nv_bfloat16, 2>(parts, d, n_q, query_start + n_requests, items, sink_scores, sink, out, stream);
     return launch_join<__nv_bfloat16, 4>(parts, d, n_q, query_start + n_requests, items, sink_scores, sink, out, stream);

@@ -34,13 +34,17 @@ struct Unit {
   int split, splits, part;
 };
 
+// The last group that starts at or before the request; called by whole warps, whose lanes look at 32 groups at once.
 __device__ __forceinline__ int group_of(const Batch& b, int request) {
-  int low = 0, high = b.n_groups - 1;             // the last group that starts at or before the request
-  while (low < high) {
-    const int mid = (low + high + 1) / 2;
-    if (b.group_start[mid] <= request) low = mid; else high = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int first = 1; first < b.n_groups; first += 32) {
+    const bool starts = first + lane < b.n_groups && b.group_start[first + lane] <= request;
+    const int here = __popc(__ballot_sync(0xffffffffu, starts));
+    before += here;
+    if (here < 32) break;
   }
-  return low;
+  return before;
 }
 
 // The keys that a group reads from its first request's table: never more than that request has.
@@ -63,7 +67,7 @@ __device__ __forceinline__ Unit prefix_unit(const Batch& b, int group, int split
 __device__ __forceinline__ Unit own_unit(const Batch& b, int request, int split, const Parts& parts) {
   Unit u;
   u.token = b.query_start[request], u.token_end = b.query_start[request + 1];
-  u.key = prefix_of(b, group_of(b, request)), u.key_end = max(u.key, b.context_lens[request]);
+  u.key = max(0, b.prefix_lens[group_of(b, request)]), u.key_end = max(u.key, b.context_lens[request]);
   u.table = b.block_tables + (size_t)request * b.table_stride;
   u.split = split, u.splits = parts.own, u.part = parts.prefix + split;
   return u;
@@ -76,11 +80,14 @@ __device__ __forceinline__ Unit unit_of(const Batch& b, int index, const Parts& 
   return own_unit(b, (index - shared) / parts.own, (index - shared) % parts.own, parts);
 }
 
-// Launches of the parts on the tensor cores (attention_prefix_tcgen05.cu: prefixes; attention_prefix_mma.cu: prefixes and own keys) and whether they take
+// Launches of the parts on the tensor cores (attention_prefix_tcgen05.cu: prefixes; attention_prefix_own.cu: own keys; attention_prefix_mma.cu: both) and whether they take
 // the sizes; `beside`: see there.
 bool prefix_tcgen05_takes(int d, int group, int page_size, long long pool_rows);
 int launch_prefix_tcgen05(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int n_tokens,
                           int max_group_tokens, float scale, float softcap, int* error_flag, cudaStream_t stream);
+bool own_tma_takes(int d, int page_size, long long pool_rows);
+int launch_own_tma(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int most_tokens,
+                   float scale, float softcap, bool beside, int* error_flag, cudaStream_t stream);
 bool prefix_mma_takes(int d);
 int launch_part_mma(const void* q, const void* k_pool, const void* v_pool, const Batch& b, const Parts& parts, int d, int most_tokens, float scale,
                     float softcap, bool own, bool beside, cudaStream_t stream);
