@@ -17,6 +17,12 @@ namespace prefix {
 // lane one key of a tile of 32 for the scores and every 32nd column for the values.
 constexpr int kRows = 16, kKeys = 32, kThreads = 128;
 
+__device__ __forceinline__ float4 load_four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load_four(const __nv_bfloat16* p) {
+  const uint2 two = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(two.x << 16), __uint_as_float(two.x & 0xffff0000u), __uint_as_float(two.y << 16), __uint_as_float(two.y & 0xffff0000u));
+}
+
 // COLUMNS: columns of the values to a lane, ceil(d / 32) or more.
 template <typename T, int COLUMNS>
 __global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, Batch b,
@@ -25,6 +31,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__
   grid_dependency_launch();
   extern __shared__ __align__(16) float smem[];
   const int dp = (d + 3) / 4 * 4, ks_stride = dp + 4;
+  const bool wide = d % 4 == 0 && ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0;
   float* q_s = smem;                                 // [kRows][dp]
   float* k_s = q_s + kRows * dp;                     // [kKeys][dp + 4]
   float* v_s = k_s + kKeys * ks_stride;              // [kKeys][dp]
@@ -55,17 +62,25 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__
   for (int tile = tile_lo; tile < tile_hi; ++tile) {
     const int key0 = u.key + tile * kKeys, live = min(kKeys, u.key_end - key0);
     __syncthreads();
-    for (int i = threadIdx.x; i < kKeys * dp; i += kThreads) {
-      const int r = i / dp, c = i % dp;
-      float k = 0.f, v = 0.f;                        // (keys behind the last are zeros: whatever their memory holds is not read)
-      if (r < live && c < d) {
-        const int key = key0 + r;
-        const size_t at = (((size_t)u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d + c;
-        k = to_float(k_pool[at]);
-        v = to_float(v_pool[at]);
+    {
+      // four threads to a key, four numbers at a time where the head size allows it; keys behind the last are zeros: whatever their memory holds is not read
+      const int r = (int)threadIdx.x / 4, key = key0 + r;
+      const size_t at = r < live ? (((size_t)u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d : 0;
+      if (wide) {
+#pragma unroll 4
+        for (int c = (int)threadIdx.x % 4 * 4; c < d; c += 16) {
+          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+          if (r < live) k = load_four(k_pool + at + c), v = load_four(v_pool + at + c);
+          *reinterpret_cast<float4*>(k_s + r * ks_stride + c) = k;
+          *reinterpret_cast<float4*>(v_s + r * dp + c) = v;
+        }
+      } else {
+        for (int c = (int)threadIdx.x % 4; c < dp; c += 4) {
+          const bool there = r < live && c < d;
+          k_s[r * ks_stride + c] = there ? to_float(k_pool[at + c]) : 0.f;
+          v_s[r * dp + c] = there ? to_float(v_pool[at + c]) : 0.f;
+        }
       }
-      k_s[r * ks_stride + c] = k;
-      v_s[i] = v;
     }
     __syncthreads();
     float s[4] = {};
@@ -282,13 +297,14 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
   const long long rows = (long long)most_tokens * group;
   int parts = 1, most = 64;
   if (tensor && !own && prefix::prefix_tcgen05_takes(d, group, page_size, 0)) {
-    // One block a multiprocessor: what costs least of the blocks' rounds times (a part's tiles + 3, about what a block takes to start and to end), and a
-    // little for every part's results.
+    // One block a multiprocessor: what costs least of the blocks' rounds times (a part's tiles, twice for two row tiles, + 4, about what a block takes to
+    // start and to end), and a little for every part's results.
     const int tokens = 128 / group;
-    const long long base = (long long)units * n_kv * ((most_tokens + tokens - 1) / tokens), tiles = (most_keys + 127) / 128;
+    const long long row_tiles = (most_tokens + tokens - 1) / tokens, base = (long long)units * n_kv * ((row_tiles + 1) / 2), tiles = (most_keys + 127) / 128;
+    const int each = row_tiles > 1 ? 2 : 1;
     double least = 1e30;
     for (int s = 1; s <= most && s <= tiles; ++s) {
-      const double cost = (double)((base * s + 147) / 148) * (double)((tiles + s - 1) / s + 3) + 0.1 * s;
+      const double cost = (double)((base * s + 147) / 148) * (double)(each * ((tiles + s - 1) / s) + 4) + 0.1 * s;
       if (cost < least) least = cost, parts = s;
     }
     return parts;
@@ -296,8 +312,8 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
   // small blocks: so many that they fill the multiprocessors, a part keeping some tiles
   const bool few = rows <= 16, ring = tensor && own && prefix::own_tma_takes(d, page_size, 0);
   const long long base = (long long)units * n_kv * (ring ? (rows <= 32 ? 1 : (rows + 63) / 64) : tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
-  const long long slots = 148 * (ring ? (few ? 12 : 6) : tensor ? (few ? 5 : 2) : 4);
-  const int keep = ring ? 128 : tensor ? (few ? 64 : 128) : 128;
+  const long long slots = 148 * (ring ? 6 : tensor ? (few ? 5 : 2) : 3);
+  const int keep = ring ? 128 : tensor ? (few ? 64 : 128) : 64;
   parts = (int)((slots + base - 1) / base);
   if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;
   if (parts > most) parts = most;
