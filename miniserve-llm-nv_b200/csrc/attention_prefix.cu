@@ -312,7 +312,7 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
   // small blocks: so many that they fill the multiprocessors, a part keeping some tiles
   const bool few = rows <= 16, ring = tensor && own && prefix::own_tma_takes(d, page_size, 0);
   const long long base = (long long)units * n_kv * (ring ? (rows <= 32 ? 1 : (rows + 63) / 64) : tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
-  const long long slots = 148 * (ring ? 6 : tensor ? (few ? 5 : 2) : 3);
+  const long long slots = 148 * (ring ? (few ? 12 : 6) : tensor ? (few ? 5 : 2) : 3);
   const int keep = ring ? 128 : tensor ? (few ? 64 : 128) : 64;
   parts = (int)((slots + base - 1) / base);
   if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;

@@ -80,6 +80,20 @@ __device__ __forceinline__ Unit unit_of(const Batch& b, int index, const Parts& 
   return own_unit(b, (index - shared) / parts.own, (index - shared) % parts.own, parts);
 }
 
+// Own keys run beside the prefixes of the same call, the kernel before theirs on the stream, which lets them start after its own wait for what came before.
+// What follows them waits for them alone: one of their blocks, the last, ends no sooner than the prefixes' kernel has.  (Where every block did,
+// each kept its place on the multiprocessor until then.)
+__device__ __forceinline__ bool last_block() {
+  return blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
+}
+
+// All of a multiprocessor's memory as shared memory while the kernel runs there, so that blocks of the prefixes and of the own keys, which need not wait for one
+// another, find room side by side.
+template <typename... Params>
+cudaError_t share_multiprocessor(void (*kernel)(Params...)) {
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 // Launches of the parts on the tensor cores (attention_prefix_tcgen05.cu: prefixes; attention_prefix_own.cu: own keys; attention_prefix_mma.cu: both) and whether they take
 // the sizes; `beside`: see there.
 bool prefix_tcgen05_takes(int d, int group, int page_size, long long pool_rows);

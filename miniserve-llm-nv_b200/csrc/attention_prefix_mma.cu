@@ -41,7 +41,7 @@ part_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict
   const int kv_head = blockIdx.y, group = b.n_q / b.n_kv;
   const int rows_total = (u.token_end - u.token) * group, row0 = (int)blockIdx.x * ROWS;
   if (row0 >= rows_total) {
-    if (beside) grid_dependency_wait();
+    if (beside && last_block()) grid_dependency_wait();
     return;
   }
   const int tiles = (u.key_end - u.key + BN - 1) / BN, share = (tiles + u.splits - 1) / u.splits;
@@ -203,7 +203,7 @@ part_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict
       if (n * 8 < d) *reinterpret_cast<float2*>(dst + n * 8 + quad_col * 2) = make_float2(acc_o[n][2 * half] * inv, acc_o[n][2 * half + 1] * inv);
     if (quad_col == 0) parts.lse[at] = l == 0.f ? -INFINITY : m_run[half] * scale_log2 + log2f(l);
   }
-  if (beside) grid_dependency_wait();
+  if (beside && last_block()) grid_dependency_wait();
 }
 
 template <int DP, int W, int BN, int STAGES>

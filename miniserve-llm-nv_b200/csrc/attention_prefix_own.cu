@@ -1,12 +1,13 @@
 // Every request's own keys behind a shared prefix, on mma.sync with TMA-fed tiles (bfloat16, head sizes 64 and 128, pages of a multiple of eight tokens).
 //
-// Thread block: W warps of 16 rows (token, query head of the key head's group) of one request and key head, over its share of the keys.  A step of single
-// tokens has one warp's rows a request; the block is then one warp, and six blocks share a multiprocessor.  Tiles of BN keys (16 KB with their values)
-// come page by page through TMA, in boxes of 8, 16 or 32 rows with the 128-byte swizzle, into a ring of two (of four for two and four
-// warps): one instruction a box where gathering the same rows took a warp 32 asynchronous copies and their addresses a tile.
-// S = Q K^T, running maximum and sum in float32, O += P V with P rounded to bfloat16 (V's type: a weight off by at most 2^-8 of itself).  Keys behind the
-// context's end are masked, their rows of V zeroed.  The reads bound it.  Waits are bounded: one that runs out sets the error flag, the copies in flight
-// land, and the block returns.
+// Thread block: W warps of 16 rows (token, query head of the key head's group) of one request and key head, over its share of the keys.  Tiles of keys
+// and values come page by page through TMA, in boxes of 8 rows and more with the 128-byte swizzle: one instruction a box where gathering the same rows
+// took a warp 32 asynchronous copies and their addresses a tile.  S = Q K^T, running maximum and sum in float32, O += P V with P rounded to
+// bfloat16 (V's type: a weight off by at most 2^-8 of itself).  Keys behind the context's end are masked, their rows of V zeroed.
+//
+// A step of single tokens has one warp's rows a request.  What such a warp waits for is itself - the fixed latencies of its own instructions, with one warp
+// on a scheduler - so blocks are small: one warp, two tiles of 8 KB, no shared memory for the rows, and twelve blocks share a multiprocessor.  The reads
+// bound it.  Waits are bounded: one that runs out sets the error flag, the copies in flight land, and the block returns.
 #include "attention_prefix.cuh"
 #include "mma_common.cuh"
 #include "tcgen05.cuh"
@@ -18,10 +19,10 @@ namespace own {
 using namespace ms::t5;
 
 template <int W> constexpr int kStages = W == 1 ? 2 : 4;
-template <int D> constexpr int kKeys = D == 128 ? 32 : 64;
+template <int D, int W> constexpr int kKeys = (D == 128 ? 16 : 32) * (W == 1 ? 1 : 2);          // of a tile
 
 template <int D, int W>
-constexpr size_t smem_bytes() { return (size_t)(16 * W) * D * 2 + (size_t)kStages<W> * 2 * kKeys<D> * D * 2 + 1024; }
+constexpr size_t smem_bytes() { return (size_t)kStages<W> * 2 * kKeys<D, W> * D * 2 + 1024; }
 
 __device__ __forceinline__ float fast_exp2(float x) {       // ex2.approx: relative error about 2^-22, -inf gives 0
   float y;
@@ -38,12 +39,11 @@ template <int D, int W>
 __global__ void __launch_bounds__(W * 32)
 own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Batch b, Parts parts,
            int box_rows, float scale_log2, float cap_log2, int beside, int* __restrict__ error_flag) {
-  constexpr int ROWS = 16 * W, THREADS = 32 * W, CHUNKS = D / 8, BN = kKeys<D>, TILE = BN * D * 2, STAGES = kStages<W>;
+  constexpr int ROWS = 16 * W, THREADS = 32 * W, CHUNKS = D / 8, BN = kKeys<D, W>, TILE = BN * D * 2, STAGES = kStages<W>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   auto k_tile = [&](int s) { return smem + (size_t)s * 2 * TILE; };
   auto v_tile = [&](int s) { return smem + (size_t)s * 2 * TILE + TILE; };
-  unsigned char* q_s = smem + (size_t)STAGES * 2 * TILE;
   __shared__ uint64_t full[STAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -82,23 +82,19 @@ own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensor
   unsigned q_frag[D / 16][4];
   float acc_o[D / 8][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   if (n_tiles > 0) {
-    for (int i = tid; i < ROWS * CHUNKS; i += THREADS) {
-      const int r = i / CHUNKS, c = i % CHUNKS, row = row0 + r;
-      const bool valid = row < rows_total;
-      const __nv_bfloat16* src = q;
-      if (valid) src = q + ((size_t)(u.token + row / group) * b.n_q + kv_head * group + row % group) * D + c * 8;
-      cp_async_16(const_cast<unsigned char*>(chunk(q_s, ROWS, r, c)), src, valid);
-    }
-    cp_async_commit();
+    // the rows straight into the fragments of the products: rows lane / 4 and 8 behind, columns 2 (lane % 4) and 8 behind of every sixteen
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int row = row0 + warp * 16 + quad_row + half * 8;
-      limit[half] = row < rows_total ? min(b.positions[u.token + row / group], u.key_end - 1) : -1;
-    }
-    cp_async_wait<0>();
-    __syncthreads();
+      const bool valid = row < rows_total;
+      limit[half] = valid ? min(b.positions[u.token + row / group], u.key_end - 1) : -1;
+      const unsigned* src = reinterpret_cast<const unsigned*>(q) + (valid ? ((size_t)(u.token + row / group) * b.n_q + kv_head * group + row % group) * (D / 2) + quad_col : 0);
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) ldmatrix_x4(q_frag[kk], chunk(q_s, ROWS, warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kk * 2 + (lane >> 4)));
+      for (int kk = 0; kk < D / 16; ++kk) {
+        q_frag[kk][half] = valid ? src[kk * 8] : 0u;
+        q_frag[kk][half + 2] = valid ? src[kk * 8 + 4] : 0u;
+      }
+    }
   }
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
@@ -222,7 +218,7 @@ own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensor
       if (quad_col == 0) parts.lse[at] = l == 0.f ? -INFINITY : m_run[half] * scale_log2 + log2f(l);
     }
   }
-  if (beside) grid_dependency_wait();
+  if (beside && last_block()) grid_dependency_wait();
 }
 
 // Rows of a page that one box takes, 0 where these pages are not taken: a power of two up to a tile that divides the page.
@@ -237,7 +233,7 @@ int launch(const void* q, const void* k_pool, const void* v_pool, int n_pages, c
            float softcap, bool beside, int* error_flag, cudaStream_t stream) {
   EncodeTiled fn = encode_tiled();
   MS_REQUIRE(fn != nullptr, "prefix attention: the driver offers no tensor maps");
-  const int box_rows = box_rows_of(b.page_size, kKeys<D>);
+  const int box_rows = box_rows_of(b.page_size, kKeys<D, W>);
   CUtensorMap map_k, map_v;
   const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)n_pages * b.n_kv * b.page_size};
   const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
@@ -249,7 +245,7 @@ int launch(const void* q, const void* k_pool, const void* v_pool, int n_pages, c
   MS_REQUIRE(encode(&map_k, k_pool) && encode(&map_v, v_pool), "prefix attention: tensor map of the pools failed");
   auto kernel = own_kernel<D, W>;
   const size_t smem = smem_bytes<D, W>();
-  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
+  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
   const long long tiles = ((long long)most_tokens * (b.n_q / b.n_kv) + 16 * W - 1) / (16 * W), units = (long long)b.n_requests * parts.own;
   MS_REQUIRE(tiles <= 2147483647LL && units <= 65535 && b.n_kv <= 65535, "prefix attention: grid %lld x %d x %lld exceeds the launch limits", tiles, b.n_kv, units);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e, twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;
@@ -271,7 +267,7 @@ int launch_rows(const void* q, const void* k_pool, const void* v_pool, int n_pag
 }  // namespace own
 
 bool own_tma_takes(int d, int page_size, long long pool_rows) {
-  return (d == 128 || d == 64) && own::box_rows_of(page_size, d == 128 ? 32 : 64) > 0 && pool_rows < 2147483648LL;
+  return (d == 128 || d == 64) && own::box_rows_of(page_size, 16) > 0 && pool_rows < 2147483648LL;
 }
 
 int launch_own_tma(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int most_tokens,

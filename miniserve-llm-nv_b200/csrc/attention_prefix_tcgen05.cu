@@ -44,14 +44,14 @@ __device__ __forceinline__ float fast_exp2(float x) {       // ex2.approx: relat
 
 template <int D, bool TWO>
 struct Layout {
-  static constexpr int K_STAGES = TWO ? 3 : 2, V_STAGES = 2;
+  static constexpr int K_STAGES = 2, V_STAGES = 2;
   static constexpr int DBLOCKS = D / 64;                 // 128-byte column blocks of a row
   static constexpr int Q_BYTES = ROWS * D * 2;           // of a row tile
   static constexpr int TILE_BYTES = BN * D * 2;          // one K or V tile
   static constexpr int K_AT = (TWO ? 2 : 1) * Q_BYTES, V_AT = K_AT + K_STAGES * TILE_BYTES;
   static constexpr size_t TOTAL = (size_t)V_AT + (size_t)V_STAGES * TILE_BYTES + 1024;
-  static constexpr int STRIDE = D + 4;                   // floats of a row of the results on their way out, over the key and value tiles
-  static_assert((TWO ? 2 : 1) * ROWS * STRIDE * 4 + ROWS * 8 <= (K_STAGES + V_STAGES) * TILE_BYTES, "the results fit over the tiles");
+  static constexpr int STRIDE = D + 4;                   // floats of a row of the results on their way out, over the rows and tiles
+  static_assert((TWO ? 2 : 1) * ROWS * STRIDE * 4 + ROWS * 8 <= V_AT + V_STAGES * TILE_BYTES, "the results fit over rows and tiles");
 };
 
 template <int D, bool TWO>
@@ -302,16 +302,16 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         tmem_fence_before();
         mbar_arrive(&p_full[s]);
       }
-      // no product reads the tiles any more once both streams are through: they hold the results on their way out, a row to a thread
+      // no product reads the rows and tiles any more once both streams are through: they hold the results on their way out, a row to a thread
       if (ok) ok = mbar_wait(&o_full[0], 0, error_flag, 41);
       if (ok && steps_of(1) > 0) ok = mbar_wait(&o_full[1], 0, error_flag, 41);
       ok = __all_sync(0xffffffffu, ok);
-      float* own_row = reinterpret_cast<float*>(smem + L::K_AT) + (size_t)((TWO ? s * ROWS : 0) + row) * L::STRIDE;
+      float* own_row = reinterpret_cast<float*>(smem) + (size_t)((TWO ? s * ROWS : 0) + row) * L::STRIDE;
       float joined_m = -INFINITY, joined_l = 0.f;                 // stream 1's, for stream 0
       const bool joined = !TWO && n_tiles > 1;
       if (joined) {
         // one row tile: stream 1's result passes to stream 0
-        float* ends = reinterpret_cast<float*>(smem + L::K_AT) + ROWS * L::STRIDE;
+        float* ends = reinterpret_cast<float*>(smem) + ROWS * L::STRIDE;
         if (s == 1) {
           ends[2 * row] = m_used, ends[2 * row + 1] = l;
           if (ok && any) {
@@ -419,7 +419,7 @@ int launch_prefix(const void* q, const void* k_pool, const void* v_pool, int n_p
   }
   auto kernel = prefix_kernel<D, TWO>;
   const size_t smem = Layout<D, TWO>::TOTAL;
-  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
+  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e;
   const float twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;
   const cudaError_t e = ms::launch(kernel, dim3((unsigned)(TWO ? (row_tiles + 1) / 2 : row_tiles), b.n_kv, (unsigned)(b.n_groups * parts.prefix)), dim3(THREADS), smem, stream, map_q,
