@@ -289,22 +289,35 @@ using namespace ms;
 // Whether the tensor-core kernels take the sizes (bfloat16, 16-byte aligned tensors); the general kernel takes all.
 MS_EXPORT int ms_prefix_attention_on_tensor_cores(int d) { return prefix::prefix_mma_takes(d) ? 1 : 0; }
 
-// Into how many parts a unit's keys are cut.  own: the units are `units` requests with up to most_tokens tokens and most_keys keys of their own, else
-// groups and their prefixes.  tensor: on the tensor cores.
-MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int n_kv, int page_size, int units, int most_tokens, int most_keys) {
+// Whether all units, prefixes too, go through the kernel of the own keys: where a group's rows are those of one warp.  (Two requests of two heads to a
+// key head behind 512 keys: 7.6 us so, 10.1 with the prefixes on tcgen05.)
+static bool one_kernel(int tensor, int d, int n_q, int n_kv, int page_size, int max_group_tokens) {
+  return tensor && (long long)max_group_tokens * (n_q / n_kv) <= 16 && prefix::own_tma_takes(d, page_size, 0);
+}
+
+// Into how many parts a unit's keys are cut.  own: the units are n_requests requests with up to max_query_len tokens and max_suffix_len keys of their own,
+// else n_groups groups and their prefixes.  tensor: on the tensor cores.
+MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int n_kv, int page_size, int n_groups, int max_group_tokens, int max_prefix_len,
+                                        int n_requests, int max_query_len, int max_suffix_len) {
+  const int units = own ? n_requests : n_groups, most_tokens = own ? max_query_len : max_group_tokens, most_keys = own ? max_suffix_len : max_prefix_len;
   if (units < 1 || n_kv < 1 || most_keys < 1) return 1;
   const int group = n_q / n_kv;
   const long long rows = (long long)most_tokens * group;
   int parts = 1, most = 64;
+  if (!own && one_kernel(tensor, d, n_q, n_kv, page_size, max_group_tokens)) own = 1;          // (the same kernel)
   if (tensor && !own && prefix::prefix_tcgen05_takes(d, group, page_size, 0)) {
-    // One block a multiprocessor: what costs least of the blocks' rounds times (a part's tiles, twice for two row tiles, + 4, about what a block takes to
-    // start and to end), and a little for every part's results.
+    // Blocks with a multiprocessor each for the prefixes: 6.5 us to start and to end, then 1 us a key tile (1.3 a row and key tile where there are two row
+    // tiles).  The multiprocessors that they leave, and a twelfth of theirs, work at the own keys meanwhile, which alone take the time of their
+    // reads at 5.5 TB/s (half of the most that they can be), 7 us at least; when the prefixes are done, all do.
     const int tokens = 128 / group;
     const long long row_tiles = (most_tokens + tokens - 1) / tokens, base = (long long)units * n_kv * ((row_tiles + 1) / 2), tiles = (most_keys + 127) / 128;
-    const int each = row_tiles > 1 ? 2 : 1;
+    const double bytes = 0.5 * 4.0 * n_requests * (double)max_suffix_len * n_kv * d, own_us = bytes / 5.5e6 > 7.0 ? bytes / 5.5e6 : 7.0;
     double least = 1e30;
     for (int s = 1; s <= most && s <= tiles; ++s) {
-      const double cost = (double)((base * s + 147) / 148) * (double)(each * ((tiles + s - 1) / s) + 4) + 0.1 * s;
+      const long long blocks = base * s, rounds = (blocks + 147) / 148;
+      const double us = (double)rounds * (6.5 + (row_tiles > 1 ? 2.6 : 1.0) * (double)((tiles + s - 1) / s));
+      const double left = blocks < 148 ? (double)(148 - blocks) / 148.0 + 1.0 / 12.0 : 1.0 / 12.0;
+      const double rest = own_us - us * left, cost = us + (rest > 0.0 ? rest : 0.0) + 0.1 * s;
       if (cost < least) least = cost, parts = s;
     }
     return parts;
@@ -313,7 +326,7 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
   const bool few = rows <= 16, ring = tensor && own && prefix::own_tma_takes(d, page_size, 0);
   const long long base = (long long)units * n_kv * (ring ? (rows <= 32 ? 1 : (rows + 63) / 64) : tensor ? (few ? 1 : (rows + 63) / 64) : (rows + 15) / 16);
   const long long slots = 148 * (ring ? (few ? 12 : 6) : tensor ? (few ? 5 : 2) : 3);
-  const int keep = ring ? 128 : tensor ? (few ? 64 : 128) : 64;
+  const int keep = ring ? (few ? 48 : 128) : tensor ? (few ? 64 : 128) : 64;
   parts = (int)((slots + base - 1) / base);
   if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;
   if (parts > most) parts = most;
@@ -346,14 +359,17 @@ MS_EXPORT int ms_prefix_attention(int tensor, const void* q, int dtype, const vo
   if (tensor) {
     MS_REQUIRE(dtype == MS_BF16 && prefix_mma_takes(d) && error_flag != nullptr, "prefix attention: head size %d is not the tensor-core kernels'", d);
     int code = 0;
-    const bool shared = prefix_parts > 0 && n_groups > 0;
-    if (shared && prefix_tcgen05_takes(d, group, page_size, (long long)n_pages * n_kv * page_size))
+    const bool shared = prefix_parts > 0 && n_groups > 0, pool_fits = (long long)n_pages * n_kv * page_size < 2147483648LL;
+    const bool together = shared && pool_fits && one_kernel(tensor, d, n_q, n_kv, page_size, max_group_tokens);
+    if (together)
+      code = launch_own_tma(q, k_pool, v_pool, n_pages, b, parts, d, max_group_tokens, scale, softcap, true, false, error_flag, stream);
+    else if (shared && prefix_tcgen05_takes(d, group, page_size, (long long)n_pages * n_kv * page_size))
       code = launch_prefix_tcgen05(q, k_pool, v_pool, n_pages, b, parts, d, n_tokens, max_group_tokens, scale, softcap, error_flag, stream);
     else if (shared)
       code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_group_tokens, scale, softcap, false, false, stream);
-    if (code == 0 && own_tma_takes(d, page_size, (long long)n_pages * n_kv * page_size))
-      code = launch_own_tma(q, k_pool, v_pool, n_pages, b, parts, d, max_query_len, scale, softcap, shared, error_flag, stream);
-    else if (code == 0)
+    if (code == 0 && !together && own_tma_takes(d, page_size, (long long)n_pages * n_kv * page_size))
+      code = launch_own_tma(q, k_pool, v_pool, n_pages, b, parts, d, max_query_len, scale, softcap, false, shared, error_flag, stream);
+    else if (code == 0 && !together)
       code = launch_part_mma(q, k_pool, v_pool, b, parts, d, max_query_len, scale, softcap, true, shared, stream);
     if (code != 0) return code;
     if (d <= 64) return launch_join<__nv_bfloat16, 2>(parts, d, n_q, query_start + n_requests, items, sink_scores, sink, out, stream);

@@ -101,7 +101,7 @@ int launch_prefix_tcgen05(const void* q, const void* k_pool, const void* v_pool,
                           int max_group_tokens, float scale, float softcap, int* error_flag, cudaStream_t stream);
 bool own_tma_takes(int d, int page_size, long long pool_rows);
 int launch_own_tma(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int most_tokens,
-                   float scale, float softcap, bool beside, int* error_flag, cudaStream_t stream);
+                   float scale, float softcap, bool all_units, bool beside, int* error_flag, cudaStream_t stream);
 bool prefix_mma_takes(int d);
 int launch_part_mma(const void* q, const void* k_pool, const void* v_pool, const Batch& b, const Parts& parts, int d, int most_tokens, float scale,
                     float softcap, bool own, bool beside, cudaStream_t stream);

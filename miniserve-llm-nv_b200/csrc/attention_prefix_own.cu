@@ -35,10 +35,11 @@ __device__ __forceinline__ const unsigned char* chunk(const unsigned char* tile,
   return tile + (size_t)(c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+// all_units: the groups' prefixes too, in the order of unit_of.
 template <int D, int W>
 __global__ void __launch_bounds__(W * 32)
 own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Batch b, Parts parts,
-           int box_rows, float scale_log2, float cap_log2, int beside, int* __restrict__ error_flag) {
+           int box_rows, float scale_log2, float cap_log2, int all_units, int beside, int* __restrict__ error_flag) {
   constexpr int ROWS = 16 * W, THREADS = 32 * W, CHUNKS = D / 8, BN = kKeys<D, W>, TILE = BN * D * 2, STAGES = kStages<W>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -56,7 +57,7 @@ own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensor
   grid_dependency_launch();
 
   const int kv_head = blockIdx.y, group = b.n_q / b.n_kv;
-  const Unit u = own_unit(b, (int)blockIdx.z / parts.own, (int)blockIdx.z % parts.own, parts);
+  const Unit u = all_units ? unit_of(b, (int)blockIdx.z, parts) : own_unit(b, (int)blockIdx.z / parts.own, (int)blockIdx.z % parts.own, parts);
   const int rows_total = (u.token_end - u.token) * group, row0 = (int)blockIdx.x * ROWS;
   // tiles from a multiple of BN on, so that a box never leaves its page; keys before the first own one are masked
   const int base = u.key / BN * BN, tiles = u.key_end > u.key ? (u.key_end - base + BN - 1) / BN : 0, share = (tiles + u.splits - 1) / u.splits;
@@ -230,7 +231,7 @@ static int box_rows_of(int page_size, int keys) {
 
 template <int D, int W>
 int launch(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int most_tokens, float scale,
-           float softcap, bool beside, int* error_flag, cudaStream_t stream) {
+           float softcap, bool all_units, bool beside, int* error_flag, cudaStream_t stream) {
   EncodeTiled fn = encode_tiled();
   MS_REQUIRE(fn != nullptr, "prefix attention: the driver offers no tensor maps");
   const int box_rows = box_rows_of(b.page_size, kKeys<D, W>);
@@ -246,22 +247,22 @@ int launch(const void* q, const void* k_pool, const void* v_pool, int n_pages, c
   auto kernel = own_kernel<D, W>;
   const size_t smem = smem_bytes<D, W>();
   MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
-  const long long tiles = ((long long)most_tokens * (b.n_q / b.n_kv) + 16 * W - 1) / (16 * W), units = (long long)b.n_requests * parts.own;
+  const long long tiles = ((long long)most_tokens * (b.n_q / b.n_kv) + 16 * W - 1) / (16 * W), units = (long long)b.n_requests * parts.own + (all_units ? (long long)b.n_groups * parts.prefix : 0);
   MS_REQUIRE(tiles <= 2147483647LL && units <= 65535 && b.n_kv <= 65535, "prefix attention: grid %lld x %d x %lld exceeds the launch limits", tiles, b.n_kv, units);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e, twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;
   const cudaError_t e = ms::launch(kernel, dim3((unsigned)tiles, b.n_kv, (unsigned)units), dim3(W * 32), smem, stream, (const __nv_bfloat16*)q, map_k, map_v, b,
-                                   parts, box_rows, scale_log2, twice, beside ? 1 : 0, error_flag);
+                                   parts, box_rows, scale_log2, twice, all_units ? 1 : 0, beside ? 1 : 0, error_flag);
   if (e != cudaSuccess) MS_FAIL("prefix attention: launch failed: %s", cudaGetErrorString(e));
   return 0;
 }
 
 template <int D>
 int launch_rows(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int most_tokens, float scale,
-                float softcap, bool beside, int* error_flag, cudaStream_t stream) {
+                float softcap, bool all_units, bool beside, int* error_flag, cudaStream_t stream) {
   const long long rows = (long long)most_tokens * (b.n_q / b.n_kv);
-  if (rows <= 16) return launch<D, 1>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, beside, error_flag, stream);
-  if (rows <= 32) return launch<D, 2>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, beside, error_flag, stream);
-  return launch<D, 4>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, beside, error_flag, stream);
+  if (rows <= 16) return launch<D, 1>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, all_units, beside, error_flag, stream);
+  if (rows <= 32) return launch<D, 2>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, all_units, beside, error_flag, stream);
+  return launch<D, 4>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, all_units, beside, error_flag, stream);
 }
 
 }  // namespace own
@@ -271,9 +272,9 @@ bool own_tma_takes(int d, int page_size, long long pool_rows) {
 }
 
 int launch_own_tma(const void* q, const void* k_pool, const void* v_pool, int n_pages, const Batch& b, const Parts& parts, int d, int most_tokens,
-                   float scale, float softcap, bool beside, int* error_flag, cudaStream_t stream) {
-  return d == 128 ? own::launch_rows<128>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, beside, error_flag, stream)
-                  : own::launch_rows<64>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, beside, error_flag, stream);
+                   float scale, float softcap, bool all_units, bool beside, int* error_flag, cudaStream_t stream) {
+  return d == 128 ? own::launch_rows<128>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, all_units, beside, error_flag, stream)
+                  : own::launch_rows<64>(q, k_pool, v_pool, n_pages, b, parts, most_tokens, scale, softcap, all_units, beside, error_flag, stream);
 }
 
 }  // namespace prefix

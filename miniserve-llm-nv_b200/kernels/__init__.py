@@ -2488,9 +2488,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     lib = library()
     tensor = int(code == 1 and _asked("ms_prefix_attention_on_tensor_cores", head_dim) == 1
                  and (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16 == 0)
-    sizes = (tensor, head_dim, n_q, n_kv, page_size)
-    prefix_parts = _asked("ms_prefix_attention_parts", 0, *sizes, n_groups, max_group_tokens, max_prefix_len) if max_prefix_len > 0 else 0
-    own_parts = _asked("ms_prefix_attention_parts", 1, *sizes, n_requests, max_query_len, max_suffix_len)
+    sizes = (tensor, head_dim, n_q, n_kv, page_size, n_groups, max_group_tokens, max_prefix_len, n_requests, max_query_len, max_suffix_len)
+    prefix_parts = _asked("ms_prefix_attention_parts", 0, *sizes) if max_prefix_len > 0 else 0
+    own_parts = _asked("ms_prefix_attention_parts", 1, *sizes)
     parts = prefix_parts + own_parts
     rows = n * n_q * parts
     scratch = torch.empty(rows * (head_dim + 1), dtype=torch.float32, device=q.device)        # (outputs of the parts, then their log-sum-exps)
