@@ -35,6 +35,7 @@ class RequestCache:
     length: int = 0
     tables: list[list[int]] = field(default_factory=list)   # per paged group: page per page index, or RELEASED
     changes: int = 0        # counts what changed committed pages (dropped or moved ones): who keeps a copy of a table looks at it
+    shared_seen: Optional[tuple] = field(default=None, repr=False, compare=False)     # the last answer of CacheManager.shared_pages
 
 
 @dataclass
@@ -205,6 +206,23 @@ class CacheManager:
             del table[keep:]
         entry.length = length
         entry.changes += 1
+
+    def shared_pages(self, request_id: str, other_id: str) -> tuple[int, ...]:
+        """Per paged group: how many leading full pages the two requests' tables have in common.  (Pages come to be shared at a fork and at the
+        attachment of a prefix, never later: the answer for a pair holds until either drops or moves pages.)"""
+        entry, other = self.requests[request_id], self.requests[other_id]
+        seen = entry.shared_seen
+        if seen is not None and seen[0] is other and seen[1:3] == (entry.changes, other.changes):
+            return seen[3]
+        full = min(entry.length, other.length) // self.page_size
+        counts = []
+        for table, others in zip(entry.tables, other.tables):
+            count = full
+            if table[:full] != others[:full]:
+                count = next(i for i in range(full) if table[i] != others[i])
+            counts.append(count)
+        entry.shared_seen = (other, entry.changes, other.changes, tuple(counts))
+        return entry.shared_seen[3]
 
     # ------------------------------------------------------------------ forks and moves
     def fork(self, request_id: str, new_ids: Sequence[str]) -> list[PageCopies]:

@@ -90,7 +90,8 @@ class CacheStorage:
         if isinstance(need, PagedKVNeed):
             block_tables, slots = ctx.group_views[self.paged_index[plan.group]]
             return PagedKVView(self.key_pools[plan.group][plan.slot], self.value_pools[plan.group][plan.slot],
-                               block_tables, slots, self.page_size, plan.writable)
+                               block_tables, slots, self.page_size, plan.writable,
+                               ctx.shared_prefixes[self.paged_index[plan.group]] if ctx.shared_prefixes else None)
         if isinstance(need, PagedLatentNeed):
             block_tables, slots = ctx.group_views[self.paged_index[plan.group]]
             return PagedLatentView(self.key_pools[plan.group][plan.slot], block_tables, slots, self.page_size, plan.writable)

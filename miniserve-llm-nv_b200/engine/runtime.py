@@ -98,7 +98,8 @@ def build_runtime(model_dir: Union[str, Path, None], engine_config: Optional[Eng
     manager = CacheManager(model.cache_groups, page_size, num_pages, engine_config.max_num_seqs,
                            engine_config.enable_prefix_cache, engine_config.prefix_cache_max_entries, namespace)
     step_function = StepFunction(model, storage, manager, max_model_len,
-                                 use_graphs=engine_config.decode_execution == "cuda_graph")
+                                 use_graphs=engine_config.decode_execution == "cuda_graph",
+                                 shared_prefixes=engine_config.shared_prefix_attention)
     resolved = replace(engine_config, max_model_len=max_model_len, num_kv_blocks=num_pages)
     chosen = _report_attention_kernels(model, dtype, page_size)
     return Runtime(config, resolved, model, storage, manager, step_function, max_model_len, report, chosen)

@@ -18,7 +18,8 @@ import torch
 
 from .. import kernels
 from ..cache.manager import RELEASED, CacheManager, StepReservation
-from ..parts.context import StepContext
+from ..parts.base import PagedKVNeed
+from ..parts.context import SharedPrefixes, StepContext
 
 
 @dataclass
@@ -31,6 +32,10 @@ class StepEntry:
 
 
 DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
+
+# With ``shared_prefixes``: keys of a prefix from which on requests form a group, and keys that need not be read a second time from which on a step
+# goes that way - one that runs eagerly anyway, and one that a captured graph would run (whose launches cost the host nothing).
+SHARED_KEYS_LEAST, SHARED_KEYS_EAGER, SHARED_KEYS_REPLAYED = 128, 512, 65536
 
 
 class DecodeGraph:
@@ -122,8 +127,10 @@ class DecodeGraph:
 
 
 class StepFunction:
-    def __init__(self, model, storage, manager: CacheManager, max_model_len: int, use_graphs: bool = False) -> None:
+    def __init__(self, model, storage, manager: CacheManager, max_model_len: int, use_graphs: bool = False,
+                 shared_prefixes: bool = False) -> None:
         self.model, self.storage, self.manager = model, storage, manager
+        self.shared_prefixes = shared_prefixes
         self.max_model_len = max_model_len
         self.device = model.device
         self.vocab_size = model.spec.vocab_size
@@ -217,8 +224,13 @@ class StepFunction:
         group_views = []
         for group in range(n_groups):
             group_views.append((views[7 + 2 * group].view(r, width), views[8 + 2 * group]))
+        shared_prefixes = []
+        if self.shared_prefixes:
+            sharing = [self._shared_groups([e.request_id for e in entries], group, SHARED_KEYS_EAGER) for group in range(n_groups)]
+            if any(found is not None for found in sharing):
+                shared_prefixes = [None if found is None else self._share(found, query_start, context_lens) for found in sharing]
         return StepContext(
-            n_tokens=n, n_requests=r, token_ids=views[0], positions=views[1], request_of_token=views[2],
+            shared_prefixes=shared_prefixes, n_tokens=n, n_requests=r, token_ids=views[0], positions=views[1], request_of_token=views[2],
             query_start=views[3], context_lens=views[4], state_slots=views[5], logit_rows=views[6],
             max_query_len=max((len(e.tokens) for e in entries), default=0),
             max_context_len=max(context_lens, default=0), dtype=self.model.dtype, device=self.device,
@@ -241,11 +253,46 @@ class StepFunction:
         """Moves the pages in use to the front of their pools."""
         self.storage.copy_pages(self.manager.compact())
 
+    # ------------------------------------------------------------------ prefixes that a step's requests share
+    def _shared_groups(self, ids: Sequence[str], group: int, least: int) -> Optional[list[tuple[int, int]]]:
+        """(requests, shared keys) of the groups that a step's requests form in one paged group, in their order; None where fewer than ``least`` keys
+        need not be read a second time, or a window or another form of cache does not allow it.  A request joins the group before it if it
+        shares more than half of that group's prefix."""
+        manager = self.manager
+        if not isinstance(manager.paged_needs[group], PagedKVNeed) or not manager.paged_needs[group].keeps_all:
+            return None
+        groups: list[list[int]] = []
+        for index, request_id in enumerate(ids):
+            common = manager.shared_pages(ids[index - 1], request_id)[group] * manager.page_size if index else 0
+            if common >= SHARED_KEYS_LEAST and (groups[-1][0] == 1 or 2 * common > groups[-1][1]):
+                groups[-1] = [groups[-1][0] + 1, min(groups[-1][1], common) if groups[-1][0] > 1 else common]
+            else:
+                groups.append([1, 0])
+        if sum((count - 1) * keys for count, keys in groups) < least:
+            return None
+        return [(count, keys) for count, keys in groups]
+
+    def _share(self, groups: Sequence[tuple[int, int]], query_start: Sequence[int], context_lens: Sequence[int]) -> SharedPrefixes:
+        starts, tokens, behind = [0], 0, 0
+        for count, keys in groups:
+            first = starts[-1]
+            starts.append(first + count)
+            tokens = max(tokens, query_start[first + count] - query_start[first])
+            behind = max(behind, max(context_lens[first:first + count]) - keys)
+        staging = torch.tensor(starts + [keys for _, keys in groups], dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        on_device = staging.to(self.device, non_blocking=True)
+        return SharedPrefixes(on_device[:len(starts)], on_device[len(starts):], tokens, max(keys for _, keys in groups), behind)
+
     # ------------------------------------------------------------------ running
     def replays(self, entries: Sequence[StepEntry]) -> bool:
-        """Whether these entries run as a captured graph: single tokens, all of whose logits are wanted."""
-        return bool(self.use_graphs and entries and len(entries) <= DECODE_BUCKETS[-1]
-                    and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries))
+        """Whether these entries run as a captured graph: single tokens, all of whose logits are wanted, that share no prefix long enough to be worth
+        an eager step."""
+        single = bool(self.use_graphs and entries and len(entries) <= DECODE_BUCKETS[-1]
+                      and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries))
+        if single and self.shared_prefixes and len(entries) > 1:
+            ids = [e.request_id for e in entries]
+            return all(self._shared_groups(ids, group, SHARED_KEYS_REPLAYED) is None for group in range(len(self.manager.paged_needs)))
+        return single
 
     def run(self, entries: Sequence[StepEntry], reservation: StepReservation,
             draw_index: Optional[Sequence[int]] = None, feed_back: bool = False) -> torch.Tensor:

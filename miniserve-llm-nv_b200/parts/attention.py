@@ -342,6 +342,13 @@ class Attention(Part):
     def _attend(self, q: torch.Tensor, ctx: StepContext, cache: PagedKVView, attended: torch.Tensor) -> None:
         if self.score_bias_slopes is not None and self._slopes_on_device is None:
             self._slopes_on_device = torch.tensor(self.score_bias_slopes, dtype=torch.float32, device=q.device)
+        shared = cache.shared
+        if shared is not None and self.window is None and self._slopes_on_device is None:
+            kernels.shared_prefix_attention(q, cache.key_pool, cache.value_pool, cache.block_tables, ctx.positions, ctx.query_start,
+                                            ctx.context_lens, shared.group_start, shared.prefix_lens, ctx.max_query_len,
+                                            shared.max_group_tokens, shared.max_prefix_len, shared.max_suffix_len, self.scale, attended,
+                                            self.score_softcap)
+            return
         kernels.paged_attention(q, cache.key_pool, cache.value_pool, cache.block_tables, ctx.request_of_token,
                                 ctx.positions, ctx.query_start, ctx.context_lens, ctx.max_query_len,
                                 ctx.max_context_len, self.scale, self.window, attended,
@@ -351,7 +358,7 @@ class Attention(Part):
         """Whether this step's norm, rotation and append run inside the attention kernel
         (``kernels.decode_attention_fused``): one token per request, a position encoding in that kernel's form (none,
         or half-split rotation over the whole head), no score modifiers, sizes that the kernel takes."""
-        if ctx.max_query_len != 1 or ctx.n_tokens != ctx.n_requests or fused is None:
+        if ctx.max_query_len != 1 or ctx.n_tokens != ctx.n_requests or fused is None or cache.shared is not None:
             return False
         if not kernels.decode_attention_fused_preferred(ctx.n_requests, self.head_dim, self.num_heads // self.num_kv_heads,
                                                         cache.key_pool.shape[2]):

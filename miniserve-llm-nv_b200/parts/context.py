@@ -17,6 +17,18 @@ import torch
 
 
 @dataclass
+class SharedPrefixes:
+    """Groups of consecutive requests of a step that share the pages of a prefix (``kernels.shared_prefix_attention``): ``group_start [G + 1]`` and
+    ``prefix_lens [G]`` on the device, and the step's own bounds."""
+
+    group_start: torch.Tensor
+    prefix_lens: torch.Tensor
+    max_group_tokens: int
+    max_prefix_len: int
+    max_suffix_len: int
+
+
+@dataclass
 class PagedKVView:
     """One run's keys and values: pools ``[pages, kv_heads, page_size, head_dim]`` of its layer.
 
@@ -31,6 +43,7 @@ class PagedKVView:
     slots: torch.Tensor
     page_size: int
     writable: bool = True
+    shared: Optional[SharedPrefixes] = None
 
 
 @dataclass
@@ -72,6 +85,7 @@ class StepContext:
     host_state_slots: list[int] = field(default_factory=list)
     memo: dict[Any, Any] = field(default_factory=dict)   # per-step scratch shared by parts (rotation tables)
     group_views: list[Any] = field(default_factory=list)  # per cache group: (block_tables, slots)
+    shared_prefixes: list[Optional[SharedPrefixes]] = field(default_factory=list)  # per cache group; empty: none
 
     def buffer(self, name: str, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
         """An uninitialised device tensor for a part's intermediate result, the same one for every call of a step
