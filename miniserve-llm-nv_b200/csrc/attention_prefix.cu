@@ -65,20 +65,21 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const T* __restrict__
     {
       // four threads to a key, four numbers at a time where the head size allows it; keys behind the last are zeros: whatever their memory holds is not read
       const int r = (int)threadIdx.x / 4, key = key0 + r;
-      const size_t at = r < live ? (((size_t)u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d : 0;
+      const int page = r < live ? u.table[key / b.page_size] : -1;
+      const bool there = (unsigned)page < (unsigned)b.n_pages;
+      const size_t at = there ? (((size_t)page * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d : 0;
       if (wide) {
 #pragma unroll 4
         for (int c = (int)threadIdx.x % 4 * 4; c < d; c += 16) {
           float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-          if (r < live) k = load_four(k_pool + at + c), v = load_four(v_pool + at + c);
+          if (there) k = load_four(k_pool + at + c), v = load_four(v_pool + at + c);
           *reinterpret_cast<float4*>(k_s + r * ks_stride + c) = k;
           *reinterpret_cast<float4*>(v_s + r * dp + c) = v;
         }
       } else {
         for (int c = (int)threadIdx.x % 4; c < dp; c += 4) {
-          const bool there = r < live && c < d;
-          k_s[r * ks_stride + c] = there ? to_float(k_pool[at + c]) : 0.f;
-          v_s[r * dp + c] = there ? to_float(v_pool[at + c]) : 0.f;
+          k_s[r * ks_stride + c] = there && c < d ? to_float(k_pool[at + c]) : 0.f;
+          v_s[r * dp + c] = there && c < d ? to_float(v_pool[at + c]) : 0.f;
         }
       }
     }
@@ -352,7 +353,7 @@ MS_EXPORT int ms_prefix_attention(int tensor, const void* q, int dtype, const vo
   const int group = n_q / n_kv, most = max_query_len > max_group_tokens ? max_query_len : max_group_tokens;
   const long long tiles = ((long long)most * group + kRows - 1) / kRows;
   MS_REQUIRE(units <= 65535 && n_kv <= 65535 && tiles <= 2147483647LL, "prefix attention: grid %lld x %d x %lld exceeds the launch limits", tiles, n_kv, units);
-  const Batch b{block_tables, table_stride, positions, query_start, context_lens, group_start, prefix_lens, page_size, n_q, n_kv, n_requests, n_groups};
+  const Batch b{block_tables, table_stride, positions, query_start, context_lens, group_start, prefix_lens, page_size, n_q, n_kv, n_requests, n_groups, n_tokens, n_pages};
   const Parts parts{part_o, part_lse, prefix_parts, own_parts, prefix_parts + own_parts};
   const dim3 grid((unsigned)tiles, n_kv, (unsigned)units);
   const int items = n_tokens * n_q;

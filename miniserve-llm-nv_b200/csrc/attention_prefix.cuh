@@ -16,8 +16,11 @@ struct Batch {
   const int* context_lens;
   const int* group_start;
   const int* prefix_lens;
-  int page_size, n_q, n_kv, n_requests, n_groups;
+  int page_size, n_q, n_kv, n_requests, n_groups, n_tokens, n_pages;
 };
+
+// Whatever the index arrays hold, no kernel reads or writes outside the tensors: tokens, requests and keys are cut to what there is, and a page that is not
+// in the pool reads as zeros.
 
 // Results of parts: o [items][count][d] and lse [items][count] in base 2, item = token * n_q + head; a unit's split i of a prefix is part i, of a
 // request's own keys part prefix + i.
@@ -26,6 +29,11 @@ struct Parts {
   float* lse;
   int prefix, own, count;
 };
+
+// The pool's row of a key in the page `page`, one behind the last (which a tensor map fills with zeros) for a page that is not there.
+__device__ __forceinline__ int pool_row_of(const Batch& b, int page, int kv_head, int key) {
+  return (unsigned)page < (unsigned)b.n_pages ? (page * b.n_kv + kv_head) * b.page_size + key % b.page_size : b.n_pages * b.n_kv * b.page_size;
+}
 
 struct Unit {
   int token, token_end;      // the rows' tokens
@@ -47,18 +55,16 @@ __device__ __forceinline__ int group_of(const Batch& b, int request) {
   return before;
 }
 
-// The keys that a group reads from its first request's table: never more than that request has.
-__device__ __forceinline__ int prefix_of(const Batch& b, int group) {
-  const int leader = b.group_start[group];
-  const int most = leader < b.n_requests ? b.context_lens[leader] : 0;
-  return max(0, min(b.prefix_lens[group], most));
-}
+__device__ __forceinline__ int within(int value, int most) { return min(max(value, 0), most); }
+// The keys of a request: never more than its table's row has room for.
+__device__ __forceinline__ int keys_of(const Batch& b, int request) { return (int)min((long long)b.context_lens[request], (long long)b.table_stride * b.page_size); }
 
 __device__ __forceinline__ Unit prefix_unit(const Batch& b, int group, int split, const Parts& parts) {
   Unit u;
-  const int first = b.group_start[group], last = min(b.group_start[group + 1], b.n_requests);
-  u.token = b.query_start[first], u.token_end = max(u.token, b.query_start[last]);
-  u.key = 0, u.key_end = prefix_of(b, group);
+  const int first = within(b.group_start[group], b.n_requests), last = within(b.group_start[group + 1], b.n_requests);
+  u.token = within(b.query_start[first], b.n_tokens), u.token_end = max(u.token, within(b.query_start[last], b.n_tokens));
+  // (never more than its first request, whose table is read, has)
+  u.key = 0, u.key_end = first < b.n_requests ? max(0, min(b.prefix_lens[group], keys_of(b, first))) : 0;
   u.table = b.block_tables + (size_t)first * b.table_stride;
   u.split = split, u.splits = parts.prefix, u.part = split;
   return u;
@@ -66,8 +72,8 @@ __device__ __forceinline__ Unit prefix_unit(const Batch& b, int group, int split
 
 __device__ __forceinline__ Unit own_unit(const Batch& b, int request, int split, const Parts& parts) {
   Unit u;
-  u.token = b.query_start[request], u.token_end = b.query_start[request + 1];
-  u.key = max(0, b.prefix_lens[group_of(b, request)]), u.key_end = max(u.key, b.context_lens[request]);
+  u.token = within(b.query_start[request], b.n_tokens), u.token_end = max(u.token, within(b.query_start[request + 1], b.n_tokens));
+  u.key = max(0, b.prefix_lens[group_of(b, request)]), u.key_end = max(u.key, keys_of(b, request));
   u.table = b.block_tables + (size_t)request * b.table_stride;
   u.split = split, u.splits = parts.own, u.part = parts.prefix + split;
   return u;

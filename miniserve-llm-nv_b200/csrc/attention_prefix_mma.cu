@@ -52,7 +52,10 @@ part_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict
     for (int r = tid; r < BN; r += THREADS) {
       const int key = key0 + r;
       long long offset = -1;
-      if (tile < tile_hi && key < u.key_end) offset = (((long long)u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d;
+      if (tile < tile_hi && key < u.key_end) {
+        const int page = u.table[key / b.page_size];
+        if ((unsigned)page < (unsigned)b.n_pages) offset = (((long long)page * b.n_kv + kv_head) * b.page_size + key % b.page_size) * d;
+      }
       row_offset[buffer * BN + r] = offset;
     }
   };

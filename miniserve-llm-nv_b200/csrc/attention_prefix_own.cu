@@ -70,7 +70,7 @@ own_kernel(const __nv_bfloat16* __restrict__ q, const __grid_constant__ CUtensor
     __syncwarp();
     for (int i = lane; i < live * (D / 64) * 2; i += 32) {
       const int values = i & 1, db = (i >> 1) % (D / 64), box = (i >> 1) / (D / 64), key = key0 + box * box_rows;
-      const int pool_row = (u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size;
+      const int pool_row = pool_row_of(b, u.table[key / b.page_size], kv_head, key);
       unsigned char* to = (values ? v_tile(stage) : k_tile(stage)) + (size_t)db * (BN * 128) + (size_t)(box * box_rows) * 128;
       tma_load_2d(to, values ? &map_v : &map_k, &full[stage], db * 64, pool_row);
     }

@@ -175,7 +175,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         unsigned char* to = keys ? k_stage(stage) : v_stage(stage);
         for (int i = lane; i < live_boxes * L::DBLOCKS; i += 32) {
           const int p = i / L::DBLOCKS, db = i % L::DBLOCKS, key = key0 + p * box_rows;
-          const int pool_row = (u.table[key / b.page_size] * b.n_kv + kv_head) * b.page_size + key % b.page_size;
+          const int pool_row = pool_row_of(b, u.table[key / b.page_size], kv_head, key);
           tma_load_2d(to + (size_t)db * (BN * 128) + (size_t)(p * box_rows) * 128, map, &full[stage], db * 64, pool_row);
         }
       }

@@ -314,6 +314,14 @@ __device__ int index_bound(Shared& s, cg::cluster_group& cluster, int rank, cons
   return s.bound;
 }
 
+// A request's record; argmax where there are none, or none in its slot.
+__device__ __forceinline__ Record record_of(const Record* records, int n_records, const int* slots, int request) {
+  Record rec{0.f, 1.f, 0};
+  if (records != nullptr && (unsigned)slots[request] < (unsigned)n_records) rec = records[slots[request]];
+  rec.top_p = fmaxf(rec.top_p, 0.f);
+  return rec;
+}
+
 __device__ __forceinline__ int request_of(const int* draft_start, int requests, int row) {
   int low = 0, high = requests - 1;               // the last request whose first row is not behind `row`
   while (low < high) {
@@ -785,7 +793,7 @@ __device__ __noinline__ void filter_by_bits(Shared& s, cg::cluster_group& cluste
 __global__ void __launch_bounds__(kThreads, 2)
 verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __restrict__ drafts, const int* __restrict__ draft_start, int requests,
                    int total, const float* __restrict__ uniforms, const float* __restrict__ draft_probs, const Record* __restrict__ records,
-                   const int* __restrict__ slots, Row* __restrict__ out, float* __restrict__ target_probs, int shift) {
+                   int n_records, const int* __restrict__ slots, Row* __restrict__ out, float* __restrict__ target_probs, int shift) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   grid_dependency_wait();
@@ -795,8 +803,7 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
   const int request = request_of(draft_start, requests, r);
   const int draft = r - request;                               // (the row's place among all drafts, if it has one)
   const bool drafted = draft >= 0 && draft < draft_start[request + 1] && draft < total;
-  Record rec{0.f, 1.f, 0};
-  if (records != nullptr) rec = records[slots[request]];
+  const Record rec = record_of(records, n_records, slots, request);
   const bool greedy = !(rec.temperature > 0.f);
   const bool top_k = rec.top_k > 0 && rec.top_k < vocab, top_p = rec.top_p < 1.f;
   const Part part(logits + (size_t)r * vocab, vocab, rank, ranks);
@@ -886,7 +893,7 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
 __global__ void __launch_bounds__(kThreads, 2)
 verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __restrict__ drafts, const int* __restrict__ draft_start,
                      const float* __restrict__ noise, const float* __restrict__ draft_probs, const Record* __restrict__ records,
-                     const int* __restrict__ slots, const Row* __restrict__ rows, int total, int* __restrict__ accepted,
+                     int n_records, const int* __restrict__ slots, const Row* __restrict__ rows, int total, int* __restrict__ accepted,
                      int* __restrict__ next_token) {
   __shared__ Joined s;
   grid_dependency_wait();
@@ -902,8 +909,7 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
   }
   const int r = first + request + passed;
   const Row row = rows[r];
-  Record rec{0.f, 1.f, 0};
-  if (records != nullptr) rec = records[slots[request]];
+  const Record rec = record_of(records, n_records, slots, request);
   const bool greedy = !(rec.temperature > 0.f);
   int chosen = row.best;
   if (!greedy && row.inverse > 0.f) {
@@ -1012,7 +1018,7 @@ MS_EXPORT int ms_verify_row_bytes() { return (int)sizeof(verify::Row); }
 // draft_start [requests + 1]; draft_probs [n_drafts, vocab] or null; noise [requests, vocab]; records [slots, 8] 32-bit words (temperature,
 // top_p as float, top_k) or null for argmax, slot_of_request [requests].  accepted, next_token [requests]; target_probs [n_drafts] or null.
 MS_EXPORT int ms_verify_drafts(const float* logits, int vocab, const int* drafts, const int* draft_start, int requests, int n_drafts,
-                               const float* uniforms, const float* noise, const float* draft_probs, const void* records,
+                               const float* uniforms, const float* noise, const float* draft_probs, const void* records, int n_records,
                                const int* slot_of_request, int* accepted, int* next_token, float* target_probs, void* scratch,
                                cudaStream_t stream) {
   using namespace ms::verify;
@@ -1027,9 +1033,9 @@ MS_EXPORT int ms_verify_drafts(const float* logits, int vocab, const int* drafts
   cudaError_t e = allow_shared(verify_rows_kernel, sizeof(Shared));
   if (e == cudaSuccess)
     e = launch_clusters(verify_rows_kernel, n_drafts + requests, ranks_for(n_drafts + requests, vocab), sizeof(Shared), stream, logits, vocab, drafts, draft_start, requests, n_drafts, uniforms,
-                                  draft_probs, (const Record*)records, slot_of_request, (Row*)scratch, target_probs, shift);
+                                  draft_probs, (const Record*)records, n_records, slot_of_request, (Row*)scratch, target_probs, shift);
   if (e == cudaSuccess)
-    e = launch_clusters(verify_choose_kernel, requests, ranks_for(requests, vocab), 0, stream, logits, vocab, drafts, draft_start, noise, draft_probs, (const Record*)records,
+    e = launch_clusters(verify_choose_kernel, requests, ranks_for(requests, vocab), 0, stream, logits, vocab, drafts, draft_start, noise, draft_probs, (const Record*)records, n_records,
                         slot_of_request, (const Row*)scratch, n_drafts, accepted, next_token);
   if (e != cudaSuccess) cudaGetLastError();
   MS_REQUIRE(e == cudaSuccess, "verify_drafts: launch failed: %s", cudaGetErrorString(e));

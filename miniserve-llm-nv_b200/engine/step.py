@@ -34,8 +34,11 @@ class StepEntry:
 DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 
 # With ``shared_prefixes``: keys of a prefix from which on requests form a group, and keys that need not be read a second time from which on a step
-# goes that way - one that runs eagerly anyway, and one that a captured graph would run (whose launches cost the host nothing).
-SHARED_KEYS_LEAST, SHARED_KEYS_EAGER, SHARED_KEYS_REPLAYED = 128, 512, 65536
+# goes that way - one that runs eagerly anyway, and one that a captured graph would run, whose launches cost the host nothing.  Qwen3-1.7B, bfloat16, ms
+# a step, without / with: four tokens each of 2 requests behind 512 keys 2.9 / 2.7, of 63 5.2 / 5.3, of 32 behind 8,192 6.2 / 5.0, of 63 behind 16,000
+# 18.4 / 6.8; a token each, replayed / eager and shared: 32 behind 2,048 2.7 / 4.6, 63 behind 2,048 3.7 / 5.3, 8 behind 16,000 3.5 / 3.1, 32 behind 8,192
+# 5.7 / 5.0, 63 behind 8,192 9.8 / 5.9, 63 behind 16,000 17.6 / 6.8.
+SHARED_KEYS_LEAST, SHARED_KEYS_EAGER, SHARED_KEYS_REPLAYED = 128, 512, 200_000
 
 
 class DecodeGraph:

@@ -2563,7 +2563,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, draft_start: torch
     ``uniforms`` (float32 ``[T]``) uniform in [0, 1) and ``noise`` (float32 ``[R, V]``) exponential variates the tokens are then distributed as drawn from
     p one by one.  With temperature 0 it is the argmax.  Where p - q is positive nowhere, p itself is drawn from.  ``target_probs`` (float32 ``[T]``, or None)
     receives ``p_i(drafts[i])``.  A logit that is NaN counts as masked (-inf); a row that is masked throughout accepts nothing and gives token 0;
-    a drafted token outside the vocabulary does not pass."""
+    a drafted token outside the vocabulary does not pass.  Vocabularies up to 524,288."""
     if logits.dim() != 2:
         raise KernelError(f"verify_drafts: logits {tuple(logits.shape)} are not [rows, vocabulary]")
     rows, vocab = logits.shape
@@ -2586,7 +2586,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, draft_start: torch
     scratch = torch.empty(rows * _asked("ms_verify_row_bytes"), dtype=torch.uint8, device=logits.device)
     _check(library().ms_verify_drafts(
         _ptr(logits), _i(vocab), _ptr(drafts), _ptr(draft_start), _i(requests), _i(total), _ptr(uniforms), _ptr(noise), _ptr(draft_probs),
-        _ptr(records), _ptr(slot_of_request), _ptr(accepted), _ptr(next_token), _ptr(target_probs), _ptr(scratch), _stream()))
+        _ptr(records), _i(0 if records is None else records.shape[0]), _ptr(slot_of_request), _ptr(accepted), _ptr(next_token), _ptr(target_probs), _ptr(scratch), _stream()))
 
 
 # --------------------------------------------------------------------------- sampling

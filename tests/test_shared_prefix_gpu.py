@@ -270,6 +270,29 @@ def test_long_cache_offsets_pass_32_bits():
     check(small, got)
 
 
+@pytest.mark.parametrize("dtype,d,page", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 5), (torch.bfloat16, 48, 16), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("count", [2, 12])
+def test_table_entries_behind_a_context_are_not_read(dtype, d, page, count):
+    """Entries behind a request's last page hold no page numbers at all."""
+    step = make(groups=[count, 1], prefix=[7 * page, 0], queries=[1] * (count + 1), suffix=[1 + 9 * i for i in range(count + 1)], d=d, dtype=dtype, page=page)
+    table, rows = step["block_tables"], step["context_lens"].tolist()
+    for r, length in enumerate(rows):
+        table[r, (length + page - 1) // page:] = (-1, 2 ** 31 - 1, 10 ** 6)[r % 3]
+    check(step, attend(step))
+
+
+@pytest.mark.parametrize("dtype,d,page", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 5), (torch.bfloat16, 48, 16), (torch.float32, 64, 16)])
+def test_nan_stays_with_its_request(dtype, d, page):
+    """NaN among a request's own keys makes its outputs NaN, and nobody else's."""
+    step = make(groups=[20], prefix=[10 * page], queries=[1] * 20, suffix=[page + 3] * 20, d=d, dtype=dtype, page=page)
+    step["k_pool"][step["block_tables"][4, 10].long(), :, 2] = float("nan")
+    got = attend(step)
+    assert torch.isnan(got[4]).all()
+    others = [r for r in range(20) if r != 4]
+    want, bound = expected({**step, "k_pool": torch.nan_to_num(step["k_pool"], nan=0.0)})
+    assert ((got.double() - want).abs()[others] <= bound[others]).all()
+
+
 def test_refusals():
     step = make(groups=[2], prefix=[32], queries=[1, 1], suffix=[3, 4])
     bad = [dict(q=step["q"].cpu()), dict(q=step["q"].half()), dict(k_pool=step["k_pool"].float()), dict(v_pool=step["v_pool"][:, :, :8]),
