@@ -287,19 +287,16 @@ using namespace ms;
 
 
 
-// Whether the tensor-core kernels take the sizes (bfloat16, 16-byte aligned tensors); the general kernel takes all.
-MS_EXPORT int ms_prefix_attention_on_tensor_cores(int d) { return prefix::prefix_mma_takes(d) ? 1 : 0; }
-
 // Whether all units, prefixes too, go through the kernel of the own keys: where a group's rows are those of one warp.  (Two requests of two heads to a
 // key head behind 512 keys: 7.6 us so, 10.1 with the prefixes on tcgen05.)
 static bool one_kernel(int tensor, int d, int n_q, int n_kv, int page_size, int max_group_tokens) {
   return tensor && (long long)max_group_tokens * (n_q / n_kv) <= 16 && prefix::own_tma_takes(d, page_size, 0);
 }
 
-// Into how many parts a unit's keys are cut.  own: the units are n_requests requests with up to max_query_len tokens and max_suffix_len keys of their own,
+// Into how many parts, 1 to 64, a unit's keys are cut.  own: the units are n_requests requests with up to max_query_len tokens and max_suffix_len keys of their own,
 // else n_groups groups and their prefixes.  tensor: on the tensor cores.
-MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int n_kv, int page_size, int n_groups, int max_group_tokens, int max_prefix_len,
-                                        int n_requests, int max_query_len, int max_suffix_len) {
+static int parts_of(int own, int tensor, int d, int n_q, int n_kv, int page_size, int n_groups, int max_group_tokens, int max_prefix_len,
+                    int n_requests, int max_query_len, int max_suffix_len) {
   const int units = own ? n_requests : n_groups, most_tokens = own ? max_query_len : max_group_tokens, most_keys = own ? max_suffix_len : max_prefix_len;
   if (units < 1 || n_kv < 1 || most_keys < 1) return 1;
   const int group = n_q / n_kv;
@@ -332,6 +329,16 @@ MS_EXPORT int ms_prefix_attention_parts(int own, int tensor, int d, int n_q, int
   if (most > (most_keys + keep - 1) / keep) most = (most_keys + keep - 1) / keep;
   if (parts > most) parts = most;
   return parts < 1 ? 1 : parts;
+}
+
+// What ms_prefix_attention is to be given for these sizes: whether the tensor-core kernels run (bfloat16 tensors at multiples of 16 bytes, a head size that
+// they take) times 65,536, the parts of a prefix (none where no group has one) times 256, the parts of a request's own keys.
+MS_EXPORT int ms_prefix_attention_plan(int dtype, int aligned, int d, int n_q, int n_kv, int page_size, int n_groups, int max_group_tokens, int max_prefix_len,
+                                       int n_requests, int max_query_len, int max_suffix_len) {
+  const int tensor = dtype == MS_BF16 && aligned && prefix::prefix_mma_takes(d) ? 1 : 0;
+  const int shared = max_prefix_len > 0 ? parts_of(0, tensor, d, n_q, n_kv, page_size, n_groups, max_group_tokens, max_prefix_len, n_requests, max_query_len, max_suffix_len) : 0;
+  const int own = parts_of(1, tensor, d, n_q, n_kv, page_size, n_groups, max_group_tokens, max_prefix_len, n_requests, max_query_len, max_suffix_len);
+  return tensor << 16 | shared << 8 | own;
 }
 
 // q, out [n_tokens, n_q, d] of type dtype; pools [pages, n_kv, page_size, d] of one layer; block_tables [requests, table_stride]; positions [n_tokens];

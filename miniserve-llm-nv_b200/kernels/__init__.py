@@ -135,8 +135,8 @@ def _want_all(checks: tuple) -> None:
     here = torch._C._cuda_getDevice()
     if _device_index is not None and _device_index != here:
         raise KernelError(f"the library's launches go to cuda:{_device_index}, the current device is cuda:{here}")
-    for tensor, name, dtype, shape in checks:
-        if tensor is None or (tensor.is_cuda and tensor.get_device() == here and tensor.is_contiguous() and (dtype is None or tensor.dtype is dtype)
+    for tensor, name, dtype, shape in checks:        # (get_device is -1 for a tensor that is not on a GPU)
+        if tensor is None or (tensor.get_device() == here and tensor.is_contiguous() and (dtype is None or tensor.dtype is dtype)
                               and (shape is None or tensor.shape == shape)):
             continue
         _want(tensor, name, dtype, shape)
@@ -2485,18 +2485,15 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         return
     if n_requests == 0 or n_groups == 0:
         raise KernelError(f"{n} tokens of {n_requests} requests in {n_groups} groups")
-    lib = library()
-    tensor = int(code == 1 and _asked("ms_prefix_attention_on_tensor_cores", head_dim) == 1
-                 and (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16 == 0)
-    sizes = (tensor, head_dim, n_q, n_kv, page_size, n_groups, max_group_tokens, max_prefix_len, n_requests, max_query_len, max_suffix_len)
-    prefix_parts = _asked("ms_prefix_attention_parts", 0, *sizes) if max_prefix_len > 0 else 0
-    own_parts = _asked("ms_prefix_attention_parts", 1, *sizes)
-    parts = prefix_parts + own_parts
-    rows = n * n_q * parts
+    q_ptr, k_ptr, v_ptr = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr()
+    plan = _asked("ms_prefix_attention_plan", code, int((q_ptr | k_ptr | v_ptr) % 16 == 0), head_dim, n_q, n_kv, page_size, n_groups, max_group_tokens,
+                  max_prefix_len, n_requests, max_query_len, max_suffix_len)
+    tensor, prefix_parts, own_parts = plan >> 16, plan >> 8 & 255, plan & 255
+    rows = n * n_q * (prefix_parts + own_parts)
     scratch = torch.empty(rows * (head_dim + 1), dtype=torch.float32, device=q.device)        # (outputs of the parts, then their log-sum-exps)
     part_o = scratch.data_ptr()
-    _check(lib.ms_prefix_attention(
-        tensor, q.data_ptr(), code, k_pool.data_ptr(), v_pool.data_ptr(), pages, block_tables.data_ptr(), block_tables.shape[1],
+    _check(library().ms_prefix_attention(
+        tensor, q_ptr, code, k_ptr, v_ptr, pages, block_tables.data_ptr(), block_tables.shape[1],
         positions.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(), group_start.data_ptr(), prefix_lens.data_ptr(), page_size, n_q, n_kv,
         head_dim, _f(scale), _f(softcap or 0.0), 1 if sink else 0, _ptr(sink_scores), out.data_ptr(), part_o, part_o + 4 * rows * head_dim,
         prefix_parts, own_parts, n_requests, n_groups, n, _i(max_query_len), _i(max_group_tokens), device_error_flag(q.device).data_ptr(), _stream()))
