@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(128) join_kernel(Parts parts, int d, int n_q, 
 
 // Block: one (token, head) of a head size that is a multiple of four.  Groups of d / 4 lanes take a part each, four numbers a lane, kDeep parts on their way
 // before their weights are known; the groups' sums meet in shared memory, in a fixed order.  One trip to the second-level cache for up to
-// 4 x 32 / (d / 4) x kDeep parts (a warp that took part after part waited for each: 19.5 us for 1,024 rows of 19 parts, now 4.6).
+// 4 x 32 / (d / 4) x kDeep parts (a warp that took part after part waited for each: 19.5 us for 1,024 rows of 19 parts, 5.3 so).
 constexpr int kMostParts = 128, kDeep = 5, kMostGroups = 64;
 template <typename T>
 __global__ void __launch_bounds__(128) join_wide_kernel(Parts parts, int d, int n_q, const int* __restrict__ tokens, const float* __restrict__ sink,
@@ -288,7 +288,7 @@ using namespace ms;
 
 
 // Whether all units, prefixes too, go through the kernel of the own keys: where a group's rows are those of one warp.  (Two requests of two heads to a
-// key head behind 512 keys: 7.6 us so, 10.1 with the prefixes on tcgen05.)
+// key head behind 512 keys: 8.0 us a call so, 10.1 with the prefixes on tcgen05.)
 static bool one_kernel(int tensor, int d, int n_q, int n_kv, int page_size, int max_group_tokens) {
   return tensor && (long long)max_group_tokens * (n_q / n_kv) <= 16 && prefix::own_tma_takes(d, page_size, 0);
 }

@@ -983,8 +983,9 @@ namespace ms {
 namespace verify {
 
 // Blocks to a row: many for few rows, whose latency counts, and fewer for more, so that no more clusters are asked for than find room at once (two blocks a
-// multiprocessor, a cluster's within one of the GPU's parts; 36 rows of 32,011 with filters: eight blocks each 52 us, four 27).  Rows of a
-// large vocabulary keep two, which even out what the filters of different rows take (272 rows of 151,936: one each 199 us, two 177).
+// multiprocessor, a cluster's within one of the GPU's parts).  Rows of a large vocabulary keep two, which even out what the filters of different
+// rows take.  us of both kernels with 1, 2, 4 and 8 blocks for every row and request: 4 rows of 151,936, greedy 14.8, 11.3, 9.3, 8.3; 72 rows
+// without filters 53, 33, 33, 40; 272 rows with filters 237, 182, 192, 370 (167 by this rule); 36 rows of 32,011 with filters 44, 33, 33, 54.
 static int ranks_for(int rows, int vocab) {
   if (rows <= 32) return kMostRanks;
   if (rows <= 64) return 4;
