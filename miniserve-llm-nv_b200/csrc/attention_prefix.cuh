@@ -3,6 +3,8 @@
 
 #include "common.cuh"
 
+#include <atomic>
+
 namespace ms {
 namespace prefix {
 
@@ -95,9 +97,16 @@ __device__ __forceinline__ bool last_block() {
 
 // All of a multiprocessor's memory as shared memory while the kernel runs there, so that blocks of the prefixes and of the own keys, which need not wait for one
 // another, find room side by side.
+// Asked of the driver once for each kernel and device (`asked`: a bit for each of the first 64 devices; asking twice does no harm).
 template <typename... Params>
-cudaError_t share_multiprocessor(void (*kernel)(Params...)) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+cudaError_t share_multiprocessor(void (*kernel)(Params...), std::atomic<unsigned long long>& asked) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if (e != cudaSuccess || (asked.load(std::memory_order_relaxed) & bit)) return e;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Launches of the parts on the tensor cores (attention_prefix_tcgen05.cu: prefixes; attention_prefix_own.cu: own keys; attention_prefix_mma.cu: both) and whether they take

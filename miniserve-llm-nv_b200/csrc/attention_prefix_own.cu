@@ -246,7 +246,8 @@ int launch(const void* q, const void* k_pool, const void* v_pool, int n_pages, c
   MS_REQUIRE(encode(&map_k, k_pool) && encode(&map_v, v_pool), "prefix attention: tensor map of the pools failed");
   auto kernel = own_kernel<D, W>;
   const size_t smem = smem_bytes<D, W>();
-  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
+  static std::atomic<unsigned long long> asked{0};
+  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel, asked) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
   const long long tiles = ((long long)most_tokens * (b.n_q / b.n_kv) + 16 * W - 1) / (16 * W), units = (long long)b.n_requests * parts.own + (all_units ? (long long)b.n_groups * parts.prefix : 0);
   MS_REQUIRE(tiles <= 2147483647LL && units <= 65535 && b.n_kv <= 65535, "prefix attention: grid %lld x %d x %lld exceeds the launch limits", tiles, b.n_kv, units);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e, twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;

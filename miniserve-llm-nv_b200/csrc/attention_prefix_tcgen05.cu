@@ -443,7 +443,8 @@ int launch_prefix(const void* q, const void* k_pool, const void* v_pool, int n_p
   }
   auto kernel = prefix_kernel<D, TWO>;
   const size_t smem = Layout<D, TWO>::TOTAL;
-  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
+  static std::atomic<unsigned long long> asked{0};
+  MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel, asked) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e;
   const float twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;
   const cudaError_t e = ms::launch(kernel, dim3((unsigned)(TWO ? (row_tiles + 1) / 2 : row_tiles), b.n_kv, (unsigned)(b.n_groups * parts.prefix)), dim3(THREADS), smem, stream, map_q,
