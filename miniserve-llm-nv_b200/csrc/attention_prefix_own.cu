@@ -7,7 +7,7 @@
 //
 // A step of single tokens has one warp's rows a request.  What such a warp waits for is itself - the fixed latencies of its own instructions, with one warp
 // on a scheduler - so blocks are small: one warp, two tiles of 8 KB, no shared memory for the rows, and twelve blocks share a multiprocessor.  The reads
-// bound it.  Waits are bounded: one that runs out sets the error flag, the copies in flight land, and the block returns.
+// bound it: 134 MB of 64 requests' own keys take about 27 us (5 TB/s), most of them while the prefixes' products run.  Waits are bounded: one that runs out sets the error flag, the copies in flight land, and the block returns.
 #include "attention_prefix.cuh"
 #include "mma_common.cuh"
 #include "tcgen05.cuh"

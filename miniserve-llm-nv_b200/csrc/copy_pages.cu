@@ -4,6 +4,7 @@
 // hundred kilobytes; it reads every source and writes every destination once, and memory bandwidth bounds it (one page: the launch).  The
 // page numbers are host-side bookkeeping: they travel as kernel arguments, with the launch, so that no copy to the device precedes it and a
 // captured launch keeps them.  The caller has checked that no destination is a source or is named twice, so the blocks need no order.
+// 256 pages of 32 KB in 16 layers of keys and of values: 81.4 us, 6.6 TB/s read and written together, the rate of a plain copy; one page in 28 layers, replayed: 1.7 us.
 #include "common.cuh"
 
 #include <string.h>
