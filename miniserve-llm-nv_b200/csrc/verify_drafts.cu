@@ -802,6 +802,7 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
   grid_dependency_launch();
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), r = (int)blockIdx.x / ranks;
+  cluster.barrier_arrive();          // (waited for before the first number goes into another block's shared memory: that block runs by then)
   const int request = request_of(draft_start, requests, r);
   const int draft = r - request;                               // (the row's place among all drafts, if it has one)
   const bool drafted = draft >= 0 && draft < draft_start[request + 1] && draft < total;
@@ -835,6 +836,7 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
       for (int j = 15; j >= 0; --j)
         if (again[j] == best.value) best.index = start + (j / 4) * 4 * kThreads + j % 4;
     }
+    cluster.barrier_wait();
     best = cluster_best(s, cluster, rank, best, 0);
     row.best = best.index == 0x7fffffff ? 0 : best.index;
     p = known && best.index == token ? 1.f : 0.f;
@@ -860,6 +862,7 @@ verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __res
       }
     });
     const float mine = best.value;
+    cluster.barrier_wait();
     row.top = cluster_best(s, cluster, rank, best, 0).value;
     if (row.top > -INFINITY) {                   // (else every entry is masked: no token has a probability)
       double sum = 0.0;                          // (rank 0's)
@@ -902,6 +905,7 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
   grid_dependency_launch();
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), request = (int)blockIdx.x / ranks;
+  cluster.barrier_arrive();          // (as above)
   const int first = min(max(draft_start[request], 0), total), count = min(max(draft_start[request + 1], first), total) - first;
   int passed = count;
   for (int base = 0; base < count && passed == count; base += 32) {          // (every warp for itself)
@@ -914,6 +918,7 @@ verify_choose_kernel(const float* __restrict__ logits, int vocab, const int* __r
   const Record rec = record_of(records, n_records, slots, request);
   const bool greedy = !(rec.temperature > 0.f);
   int chosen = row.best;
+  cluster.barrier_wait();
   if (!greedy && row.inverse > 0.f) {
     const bool rejected = passed < count;
     const float* x_row = logits + (size_t)r * vocab;
