@@ -11,7 +11,7 @@
 // Two kernels: over all rows of logits, then over one row of logits, draft probabilities and variates per request.  A cluster of one to eight
 // blocks works on a row; counts, masses and candidates meet in distributed shared memory.  Rows without filters and the second kernel are
 // bound by their reads (72 rows of 151,936 and 16 requests: 28.5 us replayed), rows with filters by their passes over the row and the barriers between them
-// (272 rows of 64 requests: 142 us, at a quarter of the memory rate; the second kernel 25).
+// (272 rows of 64 requests: about 115 us; the second kernel 25).
 //
 // The filters' borders.  Of up to 256 entries (top_k): the k-th largest of the threads' own largest entries is not above the k-th largest of all; what is not
 // below it is a list of little more than k, whose entries are ranked one by one.  Otherwise masses (for top_k counts too) in 256 bins of an eighth
@@ -791,19 +791,60 @@ __device__ __noinline__ void filter_by_bits(Shared& s, cg::cluster_group& cluste
   }
 }
 
-// Cluster: a row of logits.
+// Row number `place` of all in the order of what their filters cost, the dearest first: those that bins take, those that a list takes, those without
+// filters; inside of each in the order of the requests, which are as many as a block has threads, at most.
+__device__ __noinline__ void row_by_work(Shared& s, const int* draft_start, int requests, int total, int vocab, const Record* records, int n_records, const int* slots,
+                                         int place, int& request, int& r) {
+  const int t = (int)threadIdx.x, lane = t & 31, warp = t >> 5;
+  constexpr int kField = 21;                       // bits of a count of rows
+  int cost = 0, rows = 0;
+  if (t < requests) {
+    const Record rec = record_of(records, n_records, slots, t);
+    const bool top_k = rec.top_k > 0 && rec.top_k < vocab, filters = rec.temperature > 0.f && (top_k || rec.top_p < 1.f);
+    cost = !filters ? 2 : top_k && rec.top_k <= kFewKept ? 1 : 0;
+    rows = max(0, min(total, draft_start[t + 1] - draft_start[t]) + 1);
+  }
+  const unsigned long long mine = (unsigned long long)rows << (kField * cost);
+  unsigned long long before = mine, all = 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long other = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += other;
+  }
+  if (lane == 31) s.scan[warp] = before;
+  if (t == 0) s.found = requests - 1, s.bound = 0;
+  __syncthreads();
+  before -= mine;
+#pragma unroll 1
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before += all;
+    all += s.scan[w];
+  }
+  auto field = [](unsigned long long v, int c) { return (int)(v >> (kField * c)) & ((1 << kField) - 1); };
+  const int start = field(before, cost) + (cost > 0 ? field(all, 0) : 0) + (cost > 1 ? field(all, 1) : 0);
+  if (place >= start && place < start + rows) s.found = t, s.bound = place - start;          // one thread
+  __syncthreads();
+  request = s.found;
+  r = max(0, min(draft_start[request] + request + s.bound, total + requests - 1));
+}
+
+// Cluster: a row of logits; by_work: the rows that take longest first.
 __global__ void __launch_bounds__(kThreads, 2)
 verify_rows_kernel(const float* __restrict__ logits, int vocab, const int* __restrict__ drafts, const int* __restrict__ draft_start, int requests,
                    int total, const float* __restrict__ uniforms, const float* __restrict__ draft_probs, const Record* __restrict__ records,
-                   int n_records, const int* __restrict__ slots, Row* __restrict__ out, float* __restrict__ target_probs, int shift) {
+                   int n_records, const int* __restrict__ slots, Row* __restrict__ out, float* __restrict__ target_probs, int shift, int by_work) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   grid_dependency_wait();
   grid_dependency_launch();
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), r = (int)blockIdx.x / ranks;
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   cluster.barrier_arrive();          // (waited for before the first number goes into another block's shared memory: that block runs by then)
-  const int request = request_of(draft_start, requests, r);
+  int r = (int)blockIdx.x / ranks, request;
+  if (by_work)
+    row_by_work(s, draft_start, requests, total, vocab, records, n_records, slots, r, request, r);
+  else
+    request = request_of(draft_start, requests, r);
   const int draft = r - request;                               // (the row's place among all drafts, if it has one)
   const bool drafted = draft >= 0 && draft < draft_start[request + 1] && draft < total;
   const Record rec = record_of(records, n_records, slots, request);
@@ -992,11 +1033,18 @@ namespace verify {
 // Blocks to a row: many for few rows, whose latency counts, and fewer for more, so that no more clusters are asked for than find room at once (two blocks a
 // multiprocessor, a cluster's within one of the GPU's parts).  Rows of a large vocabulary keep two, which even out what the filters of different
 // rows take.  us of both kernels with 1, 2, 4 and 8 blocks for every row and request: 4 rows of 151,936, greedy 14.8, 11.3, 9.3, 8.3; 72 rows
-// without filters 53, 33, 33, 40; 272 rows with filters 237, 182, 192, 370 (167 by this rule); 36 rows of 32,011 with filters 44, 33, 33, 54.
+// without filters 53, 33, 33, 40; 272 rows with filters, in their order, 237, 182, 192, 370 (168 by this rule); 36 rows of 32,011 with filters 44, 33, 33, 54.
 static int ranks_for(int rows, int vocab) {
   if (rows <= 32) return kMostRanks;
   if (rows <= 64) return 4;
   return rows <= 148 || vocab >= 32768 ? 2 : 1;
+}
+
+// Whether the rows that take longest go first: where not all blocks run at once (two to a multiprocessor) and rows differ.  Otherwise the last to start may be
+// a slow one, and the others' multiprocessors wait for it: 272 rows of 64 requests with four kinds of filters, replayed: 168 us in the rows' order, 141 so; the order itself costs
+// 2 to 4 us.
+static int by_work_for(int rows, int ranks, int requests, const void* records) {
+  return (long long)rows * ranks > 2 * 148 && records != nullptr && requests <= kThreads && rows < (1 << 21) ? 1 : 0;
 }
 
 template <typename... Params, typename... Args>
@@ -1038,10 +1086,11 @@ MS_EXPORT int ms_verify_drafts(const float* logits, int vocab, const int* drafts
   MS_REQUIRE(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 8 == 0, "verify_drafts: scratch is missing or not aligned");
   int shift = 62;              // masses are sums of up to `vocab` weights of at most one, in units of 2^-shift
   while (shift > 0 && ((long long)vocab >> (62 - shift)) != 0) --shift;
+  const int rows = n_drafts + requests, ranks = ranks_for(rows, vocab);
   cudaError_t e = allow_shared(verify_rows_kernel, sizeof(Shared));
   if (e == cudaSuccess)
-    e = launch_clusters(verify_rows_kernel, n_drafts + requests, ranks_for(n_drafts + requests, vocab), sizeof(Shared), stream, logits, vocab, drafts, draft_start, requests, n_drafts, uniforms,
-                                  draft_probs, (const Record*)records, n_records, slot_of_request, (Row*)scratch, target_probs, shift);
+    e = launch_clusters(verify_rows_kernel, rows, ranks, sizeof(Shared), stream, logits, vocab, drafts, draft_start, requests, n_drafts, uniforms,
+                                  draft_probs, (const Record*)records, n_records, slot_of_request, (Row*)scratch, target_probs, shift, by_work_for(rows, ranks, requests, records));
   if (e == cudaSuccess)
     e = launch_clusters(verify_choose_kernel, requests, ranks_for(requests, vocab), 0, stream, logits, vocab, drafts, draft_start, noise, draft_probs, (const Record*)records, n_records,
                         slot_of_request, (const Row*)scratch, n_drafts, accepted, next_token);

@@ -142,6 +142,13 @@ def test_filters(vocab, probabilities, settings):
     check(make([3, 0, 5, 1, 2], vocab, settings, probabilities, seed=vocab + len(settings)))
 
 
+@pytest.mark.parametrize("count,vocab", [(64, 33001), (140, 700), (512, 300), (513, 300)])
+@pytest.mark.parametrize("settings", [[(1.0, 0.9, 0), (0.0, 1.0, 0), (0.7, 1.0, 20), (1.0, 1.0, 0), (1.2, 0.95, 290)], [(1.0, 0.9, 0)], [(1.0, 1.0, 0), (1.0, 0.9, 3)]])
+def test_more_rows_than_run_at_once(count, vocab, settings):
+    """Rows are then worked at in another order than theirs; neighbouring requests differ in number of drafts and in filters."""
+    check(make([(7 * i) % 9 % 6 for i in range(count)], vocab, settings, count % 2 == 0, seed=count))
+
+
 @pytest.mark.parametrize("vocab", [33, 5000, 32011])
 @pytest.mark.parametrize("settings", [[(1.0, 1.0, 7), (1.0, 1.0, 200), (0.5, 1.0, 31)], [(1.0, 0.9, 0), (1.0, 0.5, 0), (0.7, 0.2, 0)],
                                       [(1.0, 0.9, 100), (2.0, 0.6, 20), GREEDY]])
