@@ -1031,13 +1031,16 @@ namespace ms {
 namespace verify {
 
 // Blocks to a row: many for few rows, whose latency counts, and fewer for more, so that no more clusters are asked for than find room at once (two blocks a
-// multiprocessor, a cluster's within one of the GPU's parts).  Rows of a large vocabulary keep two, which even out what the filters of different
-// rows take.  us of both kernels with 1, 2, 4 and 8 blocks for every row and request: 4 rows of 151,936, greedy 14.8, 11.3, 9.3, 8.3; 72 rows
-// without filters 53, 33, 33, 40; 272 rows with filters, in their order, 237, 182, 192, 370 (168 by this rule); 36 rows of 32,011 with filters 44, 33, 33, 54.
+// multiprocessor, a cluster's within one of the GPU's parts).  Up to 400 rows of a large vocabulary keep two, which even out what the filters of different
+// rows take; beyond, one block's rows fill the multiprocessors and there is less to exchange.  us of both kernels with 1, 2, 4 and 8 blocks for every row and
+// request, 151,936 logits: 4 rows, greedy 14.8, 11.3, 9.3, 8.3; 72 rows without filters 53, 33, 33, 40; 272 rows with four kinds of filters 195, 140, 177, 369.
+// With 1 and 2: 408 rows 226, 203, 510 rows 237, 242, 600 rows 253, 273; of 64,000 logits 272 rows 99, 78, 408 rows 115, 113, 510 rows 122, 135; of 32,768
+// logits 272 rows 65, 62, 408 rows 71, 83; 36 rows of 32,011 44, 33.  (Where all rows cost the same, one is 2 to 20 % ahead from 170 rows on: 63, 72 for 272
+// without filters.  What they cost only the GPU knows.)
 static int ranks_for(int rows, int vocab) {
   if (rows <= 32) return kMostRanks;
   if (rows <= 64) return 4;
-  return rows <= 148 || vocab >= 32768 ? 2 : 1;
+  return rows <= 148 || (rows <= 400 && vocab >= 32768) ? 2 : 1;
 }
 
 // Whether the rows that take longest go first: where not all blocks run at once (two to a multiprocessor) and rows differ.  Otherwise the last to start may be

@@ -142,7 +142,7 @@ def test_filters(vocab, probabilities, settings):
     check(make([3, 0, 5, 1, 2], vocab, settings, probabilities, seed=vocab + len(settings)))
 
 
-@pytest.mark.parametrize("count,vocab", [(64, 33001), (140, 700), (512, 300), (513, 300)])
+@pytest.mark.parametrize("count,vocab", [(64, 33001), (140, 33001), (140, 700), (512, 300), (513, 300)])
 @pytest.mark.parametrize("settings", [[(1.0, 0.9, 0), (0.0, 1.0, 0), (0.7, 1.0, 20), (1.0, 1.0, 0), (1.2, 0.95, 290)], [(1.0, 0.9, 0)], [(1.0, 1.0, 0), (1.0, 0.9, 3)]])
 def test_more_rows_than_run_at_once(count, vocab, settings):
     """Rows are then worked at in another order than theirs; neighbouring requests differ in number of drafts and in filters."""
