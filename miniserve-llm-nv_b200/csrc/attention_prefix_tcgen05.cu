@@ -47,12 +47,19 @@ __device__ __forceinline__ float fast_exp2(float x) {       // ex2.approx: relat
 // tanh(x), x = v pre, of a row's scores (twice_pre_log2 = 2 pre log2 e).  Where all of a warp's |x| are 0.35 or less, as scores well below their cap are, by
 // the series x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835, which is off by less than 2^-23 there, two numbers an instruction: the
 // exponential and the reciprocal of capped_score keep the special-function units busy twice as long as the softmax itself (a tile took
-// 3,000 to 5,000 cycles for them).
-__device__ __forceinline__ void cap_scores(float (&v)[BN], float twice_pre_log2) {
+// 3,000 to 5,000 cycles for them).  Columns behind the row's last key, `seen` (`whole`: no row of the warp has any), have no say in it, nor has
+// a row without a token (not `mine`): they may hold products of whatever shared memory held before.
+__device__ __forceinline__ void cap_scores(float (&v)[BN], float twice_pre_log2, bool whole, int seen, bool mine) {
   const float pre = twice_pre_log2 * 0.34657359027997264f;          // ln 2 / 2
   float most = 0.f;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < BN; ++i) most = fmaxf(most, fabsf(v[i]));
+    for (int i = 0; i < BN; ++i) most = fmaxf(most, fabsf(v[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < BN; ++i) most = i <= seen ? fmaxf(most, fabsf(v[i])) : most;
+  }
+  if (!mine) most = 0.f;
   if (__all_sync(0xffffffffu, most * pre <= 0.35f)) {
     const unsigned long long pre2 = pack2(pre, pre);
 #pragma unroll
@@ -83,7 +90,7 @@ struct Layout {
   static_assert((TWO ? 2 : 1) * ROWS * STRIDE * 4 + ROWS * 8 <= V_AT + V_STAGES * TILE_BYTES, "the results fit over rows and tiles");
 };
 
-template <int D, bool TWO>
+template <int D, bool TWO, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Batch b,
               Parts parts, int box_rows, float scale_log2, float cap_log2, int* __restrict__ error_flag) {
@@ -238,7 +245,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       const int row = quarter * 32 + lane, live_rows = rows_of(s), steps = steps_of(s);
       const bool mine = row < live_rows, any = quarter * 32 < live_rows;
       const int token = token0 + (TWO ? s * tokens_per_tile : 0) + (mine ? row / group : 0);
-      const int limit = mine ? min(b.positions[token], u.key_end - 1) : -1;        // the last key that the row sees
+      // the last key that the row sees (a row without a token sees all: its numbers go nowhere, and a warp that it is in need not mask for it)
+      const int limit = mine ? min(b.positions[token], u.key_end - 1) : u.key_end - 1;
       const unsigned lane_field = (unsigned)(quarter * 32) << 16;
       const unsigned s_addr = tmem_base + lane_field + s_column(s), o_addr = tmem_base + lane_field + o_column(s);
       float m_used = -INFINITY;      // the maximum that the exponents and the output are relative to
@@ -257,9 +265,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
 #pragma unroll
           for (int c = 0; c < BN; c += 32) tmem_load_32_nowait(s_addr + c, *reinterpret_cast<float(*)[32]>(&v[c]));
           tmem_load_wait();
-          if (cap_log2 > 0.f) cap_scores(v, cap_log2);
           const int seen = min(limit, key0 + live - 1) - key0;       // keys 0 .. seen of the tile are visible
-          if (!__all_sync(0xffffffffu, seen >= BN - 1)) {
+          const bool whole = __all_sync(0xffffffffu, seen >= BN - 1);
+          if (CAP) cap_scores(v, cap_log2, whole, seen, mine);
+          if (!whole) {
 #pragma unroll
             for (int i = 0; i < BN; ++i)
               if (i > seen) v[i] = -INFINITY;
@@ -443,9 +452,11 @@ int launch_prefix(const void* q, const void* k_pool, const void* v_pool, int n_p
     const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
     MS_REQUIRE(encode(&map_k, 2, k_pool, dims, strides, box) && encode(&map_v, 2, v_pool, dims, strides, box), "prefix attention: tensor map of the pools failed");
   }
-  auto kernel = prefix_kernel<D, TWO>;
+  const bool cap = softcap > 0.f;
+  auto kernel = cap ? prefix_kernel<D, TWO, true> : prefix_kernel<D, TWO, false>;
   const size_t smem = Layout<D, TWO>::TOTAL;
-  static std::atomic<unsigned long long> asked{0};
+  static std::atomic<unsigned long long> asked_of[2];
+  std::atomic<unsigned long long>& asked = asked_of[cap ? 1 : 0];
   MS_REQUIRE(allow_shared(kernel, smem) == cudaSuccess && share_multiprocessor(kernel, asked) == cudaSuccess, "prefix attention: cannot reserve %zu bytes of shared memory", smem);
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * kLog2e;
   const float twice = softcap > 0.f ? 2.f * scale / softcap * kLog2e : 0.f;

@@ -2454,7 +2454,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     ``block_tables``, ``query_start``, ``context_lens``, ``softcap`` and ``sink`` as in :func:`paged_attention`; every key of a prefix is kept
     (no window).  Upper bounds that shape the grids, which a captured launch keeps: ``max_query_len`` and ``max_group_tokens``, the
     most tokens of a request and of a group; ``max_prefix_len`` and ``max_suffix_len``, the most keys of a prefix and of a request behind it.
-    A part's share of the keys depends on these bounds, and with it the rounding of the result."""
+    A part's share of the keys depends on these bounds, and with it the rounding of the result; under a soft cap a row's also depends on the rows beside it
+    (which of two ways a tile's scores are capped in goes by all of them).  The same call gives the same bits."""
     if q.dim() != 3 or k_pool.dim() != 4 or block_tables.dim() != 2:
         raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)} are not [N, n_q, d], the pool {tuple(k_pool.shape)} is not [pages, n_kv, page_size, "
                           f"d] or the tables {tuple(block_tables.shape)} are not [requests, width]")

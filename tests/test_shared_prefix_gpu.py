@@ -308,3 +308,20 @@ def test_refusals():
         attend(step, out=torch.empty_like(step["q"][:1]))
     none = {k: (v[:0] if k in ("q", "positions") else v) for k, v in step.items()}
     assert attend(none).shape[0] == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("case", [dict(groups=[6], prefix=[600], queries=[1, 1, 2, 1, 1, 1], suffix=[25, 1, 2, 3, 100, 24], page=24),
+                                  dict(groups=[6], prefix=[2016], queries=[2] * 6, suffix=[5, 2, 9, 64, 3, 17]),
+                                  dict(groups=[60, 2], prefix=[264, 96], queries=[1] * 62, suffix=[3] * 62, heads=6, kv_heads=2, page=24)],
+                         ids=["pages of 24", "a prefix that ends inside a tile", "rows that no token fills"])
+def test_capped_bits_do_not_depend_on_earlier_work(case, d):
+    """The same call after calls that leave small and large numbers in shared memory, where keys behind a prefix and rows without a token are never loaded:
+    the same bits.  The cap is high, so that another way of rounding a score shows in the result."""
+    step, earlier = make(d=d, softcap=1000.0, **case), make(groups=[64], prefix=[8192], queries=[1] * 64, suffix=[1] * 64, d=d)
+    got = []
+    for left in (0.0, 3e4, -3e4, 0.0):
+        attend({**earlier, **{name: torch.full_like(earlier[name], left) for name in ("q", "k_pool", "v_pool")}})
+        got.append(attend(step))
+    assert all(torch.equal(other, got[0]) for other in got[1:])
+    check(step, got[0])
