@@ -63,14 +63,19 @@ class PageAllocator:
         """Gives the pages in use the lowest numbers: ``{old number: new number}`` of those that move (highest first, each to the lowest free one);
         their holders come along.  No new number is an old one of the same call."""
         used = [page for page, count in enumerate(self._refcount) if count]
-        moves: dict[int, int] = {}
         free = [page for page in range(len(used)) if not self._refcount[page]]
-        for target, page in zip(free, reversed(used)):
-            moves[page] = target
-            self._refcount[target], self._refcount[page] = self._refcount[page], 0
-        if moves:
-            self._free_heap = list(range(len(used), self.num_pages))         # (sorted: a heap)
+        moves = dict(zip(reversed(used), free))
+        self.move(moves)
         return moves
+
+    def move(self, moves: dict[int, int]) -> None:
+        """Pages in use get other numbers, ``{old: new}``: free ones, none of them twice."""
+        if len(set(moves.values())) != len(moves) or any(self._refcount[old] <= 0 or self._refcount[new] > 0 for old, new in moves.items()):
+            raise RuntimeError("only pages in use move, and to free ones")
+        for old, new in moves.items():
+            self._refcount[new], self._refcount[old] = self._refcount[old], 0
+        if moves:
+            self._free_heap = [page for page in range(self.num_pages) if not self._refcount[page]]         # (sorted: a heap)
 
     def check_invariants(self) -> None:
         free = sorted(self._free_heap)

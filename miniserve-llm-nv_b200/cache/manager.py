@@ -261,22 +261,35 @@ class CacheManager:
 
     def compact(self) -> list[PageCopies]:
         """Gives the pages in use the lowest numbers of each pool, so that a pool's first ``used_count`` pages are all that it holds (one slice to
-        save or to hand on).  Tables and cached prefixes name the new places at once; returns per paged group the copies to make before the next step."""
+        save or to hand on).  Tables and cached prefixes name the new places at once; returns per paged group the copies to make before the next step
+        (:meth:`take_back` where they cannot be made)."""
         if self._open is not None:
             raise RuntimeError("a step is open; commit or abort first")
         copies = []
         for group, allocator in enumerate(self.allocators):
             moves = allocator.compact()
             copies.append(PageCopies(list(moves), list(moves.values())))
-            if not moves:
-                continue
-            for entry in self.requests.values():
-                entry.tables[group] = [moves.get(page, page) for page in entry.tables[group]]
-                entry.changes += 1
-            if self.prefix is not None:
-                for cached in self.prefix.entries.values():
-                    cached.pages = tuple(moves.get(page, page) if g == group else page for g, page in enumerate(cached.pages))
+            self._rename(group, moves)
         return copies
+
+    def take_back(self, copies: Sequence[PageCopies]) -> None:
+        """Undoes a :meth:`compact` whose ``copies`` failed, all or some of them, before anything else used the cache: tables and cached
+        prefixes name the old places again, which no copy writes."""
+        for group, wanted in enumerate(copies):
+            moves = dict(zip(wanted.destinations, wanted.sources))
+            self.allocators[group].move(moves)
+            self._rename(group, moves)
+
+    def _rename(self, group: int, moves: dict[int, int]) -> None:
+        """Tables and cached prefixes of a group name its pages by other numbers, ``{old: new}``."""
+        if not moves:
+            return
+        for entry in self.requests.values():
+            entry.tables[group] = [moves.get(page, page) for page in entry.tables[group]]
+            entry.changes += 1
+        if self.prefix is not None:
+            for cached in self.prefix.entries.values():
+                cached.pages = tuple(moves.get(page, page) if g == group else page for g, page in enumerate(cached.pages))
 
     # ------------------------------------------------------------------ capacity
     def pages_for(self, start: int, end: int) -> int:

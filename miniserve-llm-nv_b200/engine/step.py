@@ -254,7 +254,12 @@ class StepFunction:
 
     def compact(self) -> None:
         """Moves the pages in use to the front of their pools."""
-        self.storage.copy_pages(self.manager.compact())
+        copies = self.manager.compact()
+        try:
+            self.storage.copy_pages(copies)
+        except BaseException:
+            self.manager.take_back(copies)
+            raise
 
     # ------------------------------------------------------------------ prefixes that a step's requests share
     def _shared_groups(self, ids: Sequence[str], group: int, least: int) -> Optional[list[tuple[int, int]]]:
