@@ -244,6 +244,7 @@ class StepFunction:
     def fork(self, request_id: str, new_ids: Sequence[str]) -> None:
         """Continuations of a request as it stands (samples of one prompt, drafts to compare): ``new_ids`` share its full pages and get a copy
         of the page that is partly filled.  Their sampling records are the caller's to write (``storage.reset_slot``)."""
+        new_ids = list(new_ids)
         copies = self.manager.fork(request_id, new_ids)
         try:
             self.storage.copy_pages(copies)

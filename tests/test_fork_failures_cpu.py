@@ -66,3 +66,18 @@ def test_a_compaction_that_fails_changes_nothing(after):
     for name in list(manager.requests):
         pools.write(name, [1] * 7)
     manager.check_invariants()
+
+
+@pytest.mark.parametrize("names", [lambda: ["a", "b"], lambda: iter(["a", "b"])], ids=["a list", "names that can be walked once"])
+def test_a_fork_that_fails_changes_nothing(names):
+    manager = CacheManager([FULL, OTHER], page_size=4, num_pages=20, max_seqs=4, enable_prefix_cache=True)
+    pools = Pools(manager)
+    manager.admit("p")
+    pools.write("p", list(range(10)))
+    before = held(manager)
+    with pytest.raises(RuntimeError, match="no copy"):
+        step_function(manager, Storage(pools, 1)).fork("p", names())
+    assert held(manager) == before
+    manager.check_invariants()
+    step_function(manager, Storage(pools)).fork("p", names())
+    assert all(pools.read(name, group) == list(range(10)) for name in "pab" for group in range(2))
