@@ -283,3 +283,72 @@ def test_refusals():
             kernels.verify_drafts(**{**ok, **other})
     empty = torch.zeros(0, dtype=torch.int32, device="cuda")
     kernels.verify_drafts(torch.zeros((0, 100), device="cuda"), empty, torch.zeros(1, dtype=torch.int32, device="cuda"), None, None, empty, empty.clone())
+
+
+def _numbers_on_borders(temperature, borders, most):
+    """Distances from the largest logit that float32 products round onto a border, in eighths of a temperature, while the exact product lies beside it."""
+    eighths = torch.tensor(8.0) / torch.tensor(temperature)
+    found = []
+    for border in torch.tensor(borders):
+        distance = border / eighths
+        for steps in range(-3, 4):
+            d = (distance.view(torch.int32) + steps).view(torch.float32)
+            if d * eighths == border and d.double() * eighths.double() != border.double():
+                found.append(float(d))
+    return found[::max(1, len(found) // most)][:most]
+
+
+@pytest.mark.parametrize("vocab", [1200, 40000])
+@pytest.mark.parametrize("temperature", [1.3, 0.8])
+@pytest.mark.parametrize("borders", [[40.5 + part / 256.0 for part in range(1, 256)], [part + 0.5 for part in range(12, 120)]], ids=["parts", "bins"])
+def test_masses_of_numbers_on_a_border(borders, temperature, vocab):
+    """300 equal logits in whose middle the nucleus ends, where a rounding decides which of two neighbouring bins, or parts of one, holds them; some larger and some
+    smaller ones beside them in either."""
+    settings, rows, first = [], [], []
+    g = torch.Generator().manual_seed(2)
+    for distance in _numbers_on_borders(temperature, borders, 40):
+        near = 0.4 / 256.0 * temperature / 8.0
+        x = torch.full((vocab,), -float("inf"))
+        places = torch.randperm(vocab, generator=g)[:451]
+        x[places[0]] = 0.0
+        x[places[1:51]], x[places[51:351]], x[places[351:]] = near - distance, -distance, -distance - near
+        mass = torch.exp(x.double() / struct.unpack("f", struct.pack("f", temperature))[0])
+        settings.append((temperature, float((mass[places[:51]].sum() + 150.5 * mass[places[51]]) / mass.sum()), 0))
+        rows.append(x)
+        first.append(int(places[51:351].min()))
+    count = len(rows)
+    assert count > 20
+    logits = torch.stack(rows).repeat_interleave(2, 0).cuda()
+    case = dict(logits=logits, drafts=torch.tensor(first, dtype=torch.int32).cuda(), draft_start=torch.arange(count + 1, dtype=torch.int32).cuda(),
+                uniforms=torch.full((count,), 0.9, device="cuda"), noise=torch.empty(count, vocab, device="cuda").exponential_(generator=torch.Generator("cuda").manual_seed(3)),
+                draft_probs=None, records=records_of(settings), slot_of_request=torch.arange(count, dtype=torch.int32).cuda(), settings=settings)
+    check(case)
+
+
+@pytest.mark.parametrize("settings", [[(1.0, 0.9, 0), (1.3, 0.5, 0)], [(1.0, 1.0, 20000), (0.8, 0.95, 30000)]])
+def test_flat_rows(settings):
+    """Logits that lie close together, so that an eighth of a temperature at the border holds thousands of a block's entries: few large blocks (more rows than have
+    two each) and some of equal numbers."""
+    check(make([1] * 205, 64000, settings, True, seed=12, spread=0.5))
+    check(make([1] * 205, 40000, settings, False, seed=13, spread=0.3, grid=2.0 ** -10))
+
+
+def test_flat_rows_take_no_other_way():
+    """Flat rows are searched as peaked ones are: of 408 rows, which have a block each, they may take several times as long (their search reads them again and counts
+    thousands of entries), not the twenty times that rounds over the bits of all numbers took."""
+    def time_of(spread):
+        case = make([3] * 102, 151936, [(1.0, 0.95, 0)], False, seed=14, spread=spread)
+        for _ in range(3):
+            verify(case)
+        times = []
+        for _ in range(5):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            verify(case)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return sorted(times)[2]
+
+    peaked, flat = time_of(3.0), time_of(1.0)
+    assert flat < 9.0 * peaked, f"{flat:.3f} ms, {peaked:.3f} ms where few entries hold the mass"
