@@ -41,6 +41,40 @@ DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 SHARED_KEYS_LEAST, SHARED_KEYS_EAGER, SHARED_KEYS_REPLAYED = 128, 512, 200_000
 
 
+def prefix_groups(common: Sequence[int], least: int) -> tuple[int, list[tuple[int, int]]]:
+    """Requests in their order, cut into groups of neighbours so that the most keys need not be read a second time: ``(that number, [(requests, shared
+    keys)])``.  ``common[i]``: keys that request i has in common with the one before it; a group shares the fewest of those between its
+    requests, a group of one and one that would share fewer than ``least`` nothing.
+
+    The best cut of the first requests is the best of an earlier place and one more group.  Of neighbours that all have the same number in common, a cut
+    goes to the first or the last pair (what one group wins as it moves along, the other loses), so that places between need no look."""
+    n = len(common)
+    places = [0] + [i for i in range(1, n) if i == 1 or i == n - 1 or not common[i - 1] == common[i] == common[i + 1]] + [n]
+    saved, before, shared = [0], [0], [0]
+    for at in range(1, len(places)):
+        end, fewest = places[at], None                    # fewest: between the requests of the group from places[start] to end
+        most = -1
+        for start in range(at - 1, -1, -1):
+            first = places[start]
+            if start + 1 < at:
+                fewest = common[places[start + 1]] if fewest is None else min(fewest, common[places[start + 1]])
+            elif end - first > 1:
+                fewest = common[first + 1]
+            keys = fewest if fewest is not None and fewest >= least else 0
+            value = saved[start] + (end - first - 1) * keys
+            if value > most:
+                most, source, kept = value, start, keys
+            if fewest is not None and (fewest < least or saved[start] + (end - 1) * fewest <= most):
+                break                                     # (no earlier start can be better)
+        saved.append(most), before.append(source), shared.append(kept)
+    groups, at = [], len(places) - 1
+    while at > 0:
+        count = places[at] - places[before[at]]
+        groups += [(count, shared[at])] if shared[at] else [(1, 0)] * count
+        at = before[at]
+    return saved[-1], groups[::-1]
+
+
 class DecodeGraph:
     """One captured decode step for exactly ``rows`` rows, with fixed device buffers.
 
@@ -265,21 +299,13 @@ class StepFunction:
     # ------------------------------------------------------------------ prefixes that a step's requests share
     def _shared_groups(self, ids: Sequence[str], group: int, least: int) -> Optional[list[tuple[int, int]]]:
         """(requests, shared keys) of the groups that a step's requests form in one paged group, in their order; None where fewer than ``least`` keys
-        need not be read a second time, or a window or another form of cache does not allow it.  A request joins the group before it if it
-        shares more than half of that group's prefix."""
+        need not be read a second time, or a window or another form of cache does not allow it."""
         manager = self.manager
         if not isinstance(manager.paged_needs[group], PagedKVNeed) or not manager.paged_needs[group].keeps_all:
             return None
-        groups: list[list[int]] = []
-        for index, request_id in enumerate(ids):
-            common = manager.shared_pages(ids[index - 1], request_id)[group] * manager.page_size if index else 0
-            if common >= SHARED_KEYS_LEAST and (groups[-1][0] == 1 or 2 * common > groups[-1][1]):
-                groups[-1] = [groups[-1][0] + 1, min(groups[-1][1], common) if groups[-1][0] > 1 else common]
-            else:
-                groups.append([1, 0])
-        if sum((count - 1) * keys for count, keys in groups) < least:
-            return None
-        return [(count, keys) for count, keys in groups]
+        common = [manager.shared_pages(ids[i - 1], ids[i])[group] * manager.page_size if i else 0 for i in range(len(ids))]
+        saved, groups = prefix_groups(common, SHARED_KEYS_LEAST)
+        return groups if saved >= least else None
 
     def _share(self, groups: Sequence[tuple[int, int]], query_start: Sequence[int], context_lens: Sequence[int]) -> SharedPrefixes:
         starts, tokens, behind = [0], 0, 0
