@@ -167,7 +167,9 @@ class StepFunction:
     def __init__(self, model, storage, manager: CacheManager, max_model_len: int, use_graphs: bool = False,
                  shared_prefixes: bool = False) -> None:
         self.model, self.storage, self.manager = model, storage, manager
-        self.shared_prefixes = shared_prefixes
+        # the paged groups whose steps may read shared prefixes once
+        self.sharing_groups: list[int] = [] if not shared_prefixes else sorted(
+            manager.group_index[group][1] for group in model.sharing_groups() if manager.group_index[group][0] == "paged")
         self.max_model_len = max_model_len
         self.device = model.device
         self.vocab_size = model.spec.vocab_size
@@ -262,8 +264,9 @@ class StepFunction:
         for group in range(n_groups):
             group_views.append((views[7 + 2 * group].view(r, width), views[8 + 2 * group]))
         shared_prefixes = []
-        if self.shared_prefixes:
-            sharing = [self._shared_groups([e.request_id for e in entries], group, SHARED_KEYS_EAGER) for group in range(n_groups)]
+        if self.sharing_groups:
+            ids = [e.request_id for e in entries]
+            sharing = [self._shared_groups(ids, group, SHARED_KEYS_EAGER) if group in self.sharing_groups else None for group in range(n_groups)]
             if any(found is not None for found in sharing):
                 shared_prefixes = [None if found is None else self._share(found, query_start, context_lens) for found in sharing]
         return StepContext(
@@ -324,9 +327,9 @@ class StepFunction:
         an eager step."""
         single = bool(self.use_graphs and entries and len(entries) <= DECODE_BUCKETS[-1]
                       and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries))
-        if single and self.shared_prefixes and len(entries) > 1:
+        if single and self.sharing_groups and len(entries) > 1:
             ids = [e.request_id for e in entries]
-            return all(self._shared_groups(ids, group, SHARED_KEYS_REPLAYED) is None for group in range(len(self.manager.paged_needs)))
+            return all(self._shared_groups(ids, group, SHARED_KEYS_REPLAYED) is None for group in self.sharing_groups)
         return single
 
     def run(self, entries: Sequence[StepEntry], reservation: StepReservation,

@@ -192,6 +192,12 @@ class Attention(Part):
     def cache_members(self) -> list:
         return [self, self]
 
+    @property
+    def reads_shared_prefixes(self) -> bool:
+        """Whether a view's ``shared`` prefixes are read once for their group (:meth:`_attend`): not behind a window, in the general form
+        or with a bias of the scores, whose kernels read every request's keys for it alone."""
+        return not self.general and self.window is None and self.score_bias_slopes is None
+
     def load(self, tensors: dict[str, torch.Tensor]) -> None:
         n = self.names
         self.o_weight = tensors[n["o"]]
@@ -343,7 +349,7 @@ class Attention(Part):
         if self.score_bias_slopes is not None and self._slopes_on_device is None:
             self._slopes_on_device = torch.tensor(self.score_bias_slopes, dtype=torch.float32, device=q.device)
         shared = cache.shared
-        if shared is not None and self.window is None and self._slopes_on_device is None:
+        if shared is not None and self.reads_shared_prefixes:
             kernels.shared_prefix_attention(q, cache.key_pool, cache.value_pool, cache.block_tables, ctx.positions, ctx.query_start,
                                             ctx.context_lens, shared.group_start, shared.prefix_lens, ctx.max_query_len,
                                             shared.max_group_tokens, shared.max_prefix_len, shared.max_suffix_len, self.scale, attended,

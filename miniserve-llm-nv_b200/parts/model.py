@@ -125,6 +125,21 @@ class DecoderModel:
     def cache_groups_need(keys, group):
         return keys[group]
 
+    def sharing_groups(self) -> set[int]:
+        """The cache groups of which some run's attention reads a prefix that requests share once for all of them."""
+        found: set[int] = set()
+
+        def look(plan, mixer) -> None:
+            if isinstance(plan, tuple):
+                for member_plan, member in zip(plan, mixer.cache_members()):
+                    look(member_plan, member)
+            elif plan is not None and getattr(mixer, "reads_shared_prefixes", False):
+                found.add(plan.group)
+
+        for run, plan in zip(self.spec.order, self.run_caches):
+            look(plan, self.blocks[run.layer].mixer)
+        return found
+
     # ------------------------------------------------------------------ weights
     def load(self, tensors: dict[str, torch.Tensor]) -> None:
         self.embedding = tensors[self.spec.embedding_name]
