@@ -40,6 +40,16 @@ DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 # 5.7 / 5.0, 63 behind 8,192 9.8 / 5.9, 63 behind 16,000 17.6 / 6.8.
 SHARED_KEYS_LEAST, SHARED_KEYS_EAGER, SHARED_KEYS_REPLAYED = 128, 512, 200_000
 
+# What else those keys have to outweigh, in keys: tokens of requests that bring several, whose own keys go through kernels made for few rows and whose results
+# through float32 parts (SHARED_KEYS_TOKEN for each, SHARED_KEYS_PAIR for each pair of a request's, both for each query head of a key head), and, where a request brings more than 16
+# rows to a key head, the longest way along one request's own keys, which are then not cut into parts (SHARED_KEYS_OWN for each, with eight key heads; fewer
+# read less for every key).  us of one layer's attention, without / with sharing, 16 query and 8 key heads of 128, bfloat16: eight requests behind 2,048 keys, 1
+# token each 14 / 11, 16 each 22 / 19, 64 each 23 / 39, 512 each 92 / 262; behind 8,192, 64 each 66 / 57, 256 each 132 / 203; 63 single tokens behind 2,048
+# beside another request's portion of 64 89 / 21, of 512 92 / 77, of 2,048 109 / 354; behind 8,192 beside 2,048 324 / 377.  Over 2,064 steps of six sets of
+# heads, behind 512 to 16,384 keys, the steps chosen gain 74 of the 85 ms that the faster way of each would, 37 are behind by
+# more than 5 % (0.4 ms in all, 1.57 times as long at worst); every step from SHARED_KEYS_EAGER on would have lost 174.
+SHARED_KEYS_TOKEN, SHARED_KEYS_PAIR, SHARED_KEYS_OWN = 60, 0.05, 160
+
 
 def prefix_groups(common: Sequence[int], least: int) -> tuple[int, list[tuple[int, int]]]:
     """Requests in their order, cut into groups of neighbours so that the most keys need not be read a second time: ``(that number, [(requests, shared
@@ -168,8 +178,8 @@ class StepFunction:
                  shared_prefixes: bool = False) -> None:
         self.model, self.storage, self.manager = model, storage, manager
         # the paged groups whose steps may read shared prefixes once
-        self.sharing_groups: list[int] = [] if not shared_prefixes else sorted(
-            manager.group_index[group][1] for group in model.sharing_groups() if manager.group_index[group][0] == "paged")
+        self.sharing_groups: dict[int, int] = {} if not shared_prefixes else {
+            manager.group_index[group][1]: heads for group, heads in model.sharing_groups().items() if manager.group_index[group][0] == "paged"}
         self.max_model_len = max_model_len
         self.device = model.device
         self.vocab_size = model.spec.vocab_size
@@ -267,6 +277,7 @@ class StepFunction:
         if self.sharing_groups:
             ids = [e.request_id for e in entries]
             sharing = [self._shared_groups(ids, group, SHARED_KEYS_EAGER) if group in self.sharing_groups else None for group in range(n_groups)]
+            sharing = [found if found is not None and self._outweighs(found, group, query_start, context_lens) else None for group, found in enumerate(sharing)]
             if any(found is not None for found in sharing):
                 shared_prefixes = [None if found is None else self._share(found, query_start, context_lens) for found in sharing]
         return StepContext(
@@ -309,6 +320,16 @@ class StepFunction:
         common = [manager.shared_pages(ids[i - 1], ids[i])[group] * manager.page_size if i else 0 for i in range(len(ids))]
         saved, groups = prefix_groups(common, SHARED_KEYS_LEAST)
         return groups if saved >= least else None
+
+    def _outweighs(self, groups: Sequence[tuple[int, int]], group: int, query_start: Sequence[int], context_lens: Sequence[int]) -> bool:
+        """Whether the keys that need not be read a second time outweigh what else is slower (see SHARED_KEYS_TOKEN)."""
+        heads = self.sharing_groups[group]
+        new = [end - start for start, end in zip(query_start[:-1], query_start[1:])]
+        most = heads * sum(SHARED_KEYS_TOKEN * count + SHARED_KEYS_PAIR * count * count for count in new if count > 1)
+        if max(new) * heads > 16:
+            prefix = [keys for count, keys in groups for _ in range(count)]
+            most += SHARED_KEYS_OWN * 8 / self.manager.paged_needs[group].num_kv_heads * max(length - keys for length, keys in zip(context_lens, prefix))
+        return sum((count - 1) * keys for count, keys in groups) >= most
 
     def _share(self, groups: Sequence[tuple[int, int]], query_start: Sequence[int], context_lens: Sequence[int]) -> SharedPrefixes:
         starts, tokens, behind = [0], 0, 0

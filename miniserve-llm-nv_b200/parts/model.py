@@ -125,16 +125,17 @@ class DecoderModel:
     def cache_groups_need(keys, group):
         return keys[group]
 
-    def sharing_groups(self) -> set[int]:
-        """The cache groups of which some run's attention reads a prefix that requests share once for all of them."""
-        found: set[int] = set()
+    def sharing_groups(self) -> dict[int, int]:
+        """The cache groups of which some run's attention reads a prefix that requests share once for all of them, each with the most query
+        heads to a key head among those runs."""
+        found: dict[int, int] = {}
 
         def look(plan, mixer) -> None:
             if isinstance(plan, tuple):
                 for member_plan, member in zip(plan, mixer.cache_members()):
                     look(member_plan, member)
             elif plan is not None and getattr(mixer, "reads_shared_prefixes", False):
-                found.add(plan.group)
+                found[plan.group] = max(found.get(plan.group, 0), mixer.num_heads // mixer.num_kv_heads)
 
         for run, plan in zip(self.spec.order, self.run_caches):
             look(plan, self.blocks[run.layer].mixer)

@@ -68,7 +68,7 @@ def function_of(model, shared=True):
 def test_steps_of_a_model(monkeypatch, name):
     build, groups = MODELS[name]
     model = build()
-    assert model.sharing_groups() == groups
+    assert set(model.sharing_groups()) == groups
     function = function_of(model)
     entries = [StepEntry(request, [1], [0]) for request in ("p", "a", "b")]
     assert function.replays(entries)                       # (few keys: the graph)
@@ -96,7 +96,32 @@ def test_models_of_members_name_their_groups():
     for raw in venarax_helpers.CONFIGS.values():
         architecture = resolve_architecture(raw)
         model = DecoderModel(architecture.build_spec(architecture.config_class.from_dict(raw)), torch.float32, "cpu")
-        assert model.sharing_groups() <= set(range(len(model.cache_groups)))
+        assert set(model.sharing_groups()) <= set(range(len(model.cache_groups)))
     inner = dict(hidden_size=64, inner=attention())
     model = toy(PartSpec("token_shift", inner))
     assert [model.run_caches[0][1].group] == sorted(model.sharing_groups())
+
+
+@pytest.mark.parametrize("behind,new,alone,shares", [
+    (512, [1] * 8, None, True), (512, [4] * 8, None, False), (512, [64] * 8, None, False), (512, [1] * 8, 256, False),
+    (2048, [8] * 8, None, True), (2048, [128] * 4, None, False), (2048, [1] * 30, 2, True), (2048, [1] * 30, 1024, False), (2048, [1, 1], 400, False),
+    (2048, [1500, 1], None, False), (3584, [1] * 30, 64, True)])
+def test_prompt_portions_have_to_be_outweighed(behind, new, alone, shares):
+    """Steps whose portions are long for what they share run as without the option (two query heads to a key head, eight key heads)."""
+    function = function_of_heads(behind, len(new))
+    entries = [StepEntry(f"r{i}", [1] * count, [count - 1]) for i, count in enumerate(new)]
+    if alone is not None:
+        function.manager.admit("alone")
+        entries.append(StepEntry("alone", [1] * alone, [alone - 1]))
+    reservation = function.manager.prepare([(e.request_id, len(e.tokens)) for e in entries])
+    assert bool(function.build_context(entries, reservation).shared_prefixes) == shares
+
+
+def function_of_heads(behind, count):
+    model = toy(attention(num_heads=16, num_kv_heads=8, head_dim=32))
+    manager = CacheManager(model.cache_groups, PAGE, 2000, 40)
+    function = StepFunction(model, SimpleNamespace(num_pages=2000, scratch_page=2000, scratch_slot=40), manager, 4096, shared_prefixes=True)
+    manager.admit("p")
+    manager.commit(manager.prepare([("p", behind)]))
+    manager.fork("p", [f"r{i}" for i in range(count)])
+    return function
