@@ -15,6 +15,7 @@ page depend on nothing but the tokens before it.
 
 from __future__ import annotations
 
+import itertools
 from dataclasses import dataclass, field
 
 import numpy
@@ -35,6 +36,7 @@ class RequestCache:
     length: int = 0
     tables: list[list[int]] = field(default_factory=list)   # per paged group: page per page index, or RELEASED
     changes: int = 0        # counts what changed committed pages (dropped or moved ones): who keeps a copy of a table looks at it
+    serial: int = field(default_factory=itertools.count().__next__, repr=False, compare=False)     # no two admissions have the same
     shared_seen: Optional[tuple] = field(default=None, repr=False, compare=False)     # the last answer of CacheManager.shared_pages
 
 
@@ -212,8 +214,9 @@ class CacheManager:
         attachment of a prefix, never later: the answer for a pair holds until either drops or moves pages.)"""
         entry, other = self.requests[request_id], self.requests[other_id]
         seen = entry.shared_seen
-        if seen is not None and seen[0] is other and seen[1:3] == (entry.changes, other.changes):
-            return seen[3]
+        asked = (other.serial, entry.changes, other.changes)        # (not the record: one that is released would live as long as this one)
+        if seen is not None and seen[0] == asked:
+            return seen[1]
         full = min(entry.length, other.length) // self.page_size
         counts = []
         for table, others in zip(entry.tables, other.tables):
@@ -221,8 +224,8 @@ class CacheManager:
             if table[:full] != others[:full]:
                 count = next(i for i in range(full) if table[i] != others[i])
             counts.append(count)
-        entry.shared_seen = (other, entry.changes, other.changes, tuple(counts))
-        return entry.shared_seen[3]
+        entry.shared_seen = (asked, tuple(counts))
+        return entry.shared_seen[1]
 
     # ------------------------------------------------------------------ forks and moves
     def fork(self, request_id: str, new_ids: Sequence[str]) -> list[PageCopies]:

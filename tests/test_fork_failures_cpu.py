@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import copy
+import gc
+import weakref
 
 import pytest
 
@@ -81,3 +83,27 @@ def test_a_fork_that_fails_changes_nothing(names):
     manager.check_invariants()
     step_function(manager, Storage(pools)).fork("p", names())
     assert all(pools.read(name, group) == list(range(10)) for name in "pab" for group in range(2))
+
+
+def test_released_records_do_not_live_on_in_others():
+    """A request that is kept while others come and go (a prompt that is forked) holds none of their records."""
+    manager = CacheManager([FULL], page_size=4, num_pages=60, max_seqs=8)
+    pools = Pools(manager)
+    manager.admit("p")
+    pools.write("p", list(range(12)))
+    seen, live = [], ["p"]
+    for i in range(20):                        # each new one stands behind the one before, as in the steps of a batch
+        manager.fork("p", [f"r{i}"])
+        live.append(f"r{i}")
+        for name, other in zip(live[:-1], live[1:]):
+            assert manager.shared_pages(name, other) == (3,)
+        seen.append(weakref.ref(manager.requests[f"r{i}"]))
+        if len(live) > 3:
+            manager.release(live.pop(1))
+        live = [name for name in live if name != "p"]          # (only the first time is it in a step)
+    gc.collect()
+    assert sum(record() is not None for record in seen) == len(manager.requests) - 1
+    # the same name admitted again is another request
+    manager.release("r19")
+    manager.admit("r19")
+    assert manager.shared_pages("r18", "r19") == (0,)
