@@ -2478,8 +2478,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if min(max_query_len, max_group_tokens) < 0 or min(max_prefix_len, max_suffix_len) < 0 or max_group_tokens < max_query_len:
         raise KernelError(f"shared_prefix_attention: at most {max_query_len} tokens of a request, {max_group_tokens} of a group, {max_prefix_len} keys of a "
                           f"prefix and {max_suffix_len} behind it")
-    if softcap is not None and not softcap >= 0.0:
-        raise KernelError(f"softcap {softcap} is negative")
+    if softcap is not None and not 0.0 <= softcap < math.inf:
+        raise KernelError(f"softcap {softcap} is negative or not finite")
     if not 0.0 < scale < math.inf:
         raise KernelError(f"scale {scale} is not a positive number")
     if n == 0:

@@ -325,3 +325,12 @@ def test_capped_bits_do_not_depend_on_earlier_work(case, d):
         got.append(attend(step))
     assert all(torch.equal(other, got[0]) for other in got[1:])
     check(step, got[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+def test_an_infinite_cap_is_refused(dtype):
+    """(It would multiply by infinity what tanh gave; no cap is None or 0.)"""
+    step = make(groups=[2], prefix=[32], queries=[1, 1], suffix=[3, 4], dtype=dtype)
+    with pytest.raises(KernelError):
+        attend(step, softcap=float("inf"))
+    check(step, attend(step, softcap=0.0))
