@@ -298,7 +298,7 @@ static bool one_kernel(int tensor, int d, int n_q, int n_kv, int page_size, int 
 static int parts_of(int own, int tensor, int d, int n_q, int n_kv, int page_size, int n_groups, int max_group_tokens, int max_prefix_len,
                     int n_requests, int max_query_len, int max_suffix_len) {
   const int units = own ? n_requests : n_groups, most_tokens = own ? max_query_len : max_group_tokens, most_keys = own ? max_suffix_len : max_prefix_len;
-  if (units < 1 || n_kv < 1 || most_keys < 1) return 1;
+  if (units < 1 || n_kv < 1 || most_keys < 1 || most_tokens < 1) return 1;
   const int group = n_q / n_kv;
   const long long rows = (long long)most_tokens * group;
   int parts = 1, most = 64;

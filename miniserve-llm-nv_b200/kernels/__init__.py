@@ -2482,7 +2482,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         raise KernelError(f"softcap {softcap} is negative or not finite")
     if not 0.0 < scale < math.inf:
         raise KernelError(f"scale {scale} is not a positive number")
-    if n == 0:
+    if n == 0 or max_query_len == 0:
         return
     if n_requests == 0 or n_groups == 0:
         raise KernelError(f"{n} tokens of {n_requests} requests in {n_groups} groups")

@@ -334,3 +334,17 @@ def test_an_infinite_cap_is_refused(dtype):
     with pytest.raises(KernelError):
         attend(step, softcap=float("inf"))
     check(step, attend(step, softcap=0.0))
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.bfloat16, 40), (torch.float32, 64)])
+def test_a_batch_without_any_token(dtype, d):
+    """Rows of padding alone, whose bounds say that no request brings a token: nothing is computed and nothing written."""
+    step = make(groups=[2, 1], prefix=[32, 0], queries=[0, 0, 0], suffix=[3, 4, 1], d=d, dtype=dtype)
+    step["q"] = torch.full((3, 8, d), float("nan"), dtype=dtype, device="cuda")
+    step["positions"] = torch.zeros(3, dtype=torch.int32, device="cuda")
+    out = torch.full_like(step["q"], 7.0)
+    attend(step, out)
+    assert step["max_query_len"] == 0 and (out == 7.0).all()
+    attend({**step, "max_query_len": 2, "max_group_tokens": 4}, out)
+    assert (out == 7.0).all()
+    torch.cuda.synchronize()
