@@ -17,7 +17,7 @@
 // A row tile and key tile of head size 128 are 8.4 MFLOP and 16,384 exponentials: 0.75 us of a multiprocessor's share of the measured rate of products, 0.54
 // of its exponential units; reading the key tile takes its share of the memory rate 1.45 us.  So the reads bound one row tile, the products two.
 // Measured: a step of two row tiles takes 3,950 cycles of which the products take 3,300 (104 a 128 x 128 x 16 product); 64 requests behind 32,768 keys, own
-// keys and join with them, 72 us replayed; 32 behind 4,096, where setting up, results and join (about 12 us) are most of it, 19.4.
+// keys and join with them, 71 us replayed; 32 behind 4,096, where setting up, results and join (about 12 us) are most of it, 19.5.
 // All mbarrier waits are bounded; a wait that runs out sets the error flag and every role drains and returns.
 #include "attention_prefix.cuh"
 #include "tcgen05.cuh"

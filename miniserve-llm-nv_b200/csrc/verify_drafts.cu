@@ -10,8 +10,8 @@
 //
 // Two kernels: over all rows of logits, then over one row of logits, draft probabilities and variates per request.  A cluster of one to eight
 // blocks works on a row; counts, masses and candidates meet in distributed shared memory.  Rows without filters and the second kernel are
-// bound by their reads (72 rows of 151,936 and 16 requests: 28.5 us replayed), rows with filters by their passes over the row and the barriers between them
-// (272 rows of 64 requests: about 115 us; the second kernel 25).
+// bound by their reads (72 rows of 151,936 and 16 requests: 30 us replayed), rows with filters by their passes over the row and the barriers between them
+// (272 rows of 64 requests: about 113 us; the second kernel 25).
 //
 // The filters' borders.  Of up to 256 entries (top_k): the k-th largest of the threads' own largest entries is not above the k-th largest of all; what is not
 // below it is a list of little more than k, whose entries are ranked one by one.  Otherwise masses (for top_k counts too) in 256 bins of an eighth
